@@ -136,7 +136,7 @@ def prepare(case, seed):
         st["x"] = _normal(g, (T, inn))
         st["bias"] = _normal(g, (out,), 0.1) if case["bias"] else None
         st["codes"] = _codes(g, (out // 16, nb, 2, 32, 16))
-        st["params"] = _params(g, (out // 16, nb * 128 // group, 16), 0.02)
+        st["params"] = _params(g, (out // 16, nb, 16, 128 // group), 0.02)
         if own:
             et = importlib.import_module("scpaper-2021_b200")
             st["et"] = et
@@ -397,12 +397,12 @@ def exact(case, seed):
         inn, out, group = case["in"], case["out"], case["group"]
         words = st["codes"].view(torch.int32).view(out // 16, -1, 2, 8, 4, 4)
         w = torch.empty((out // 16, 2, 8, words.shape[1] * 128), dtype=F64, device="cuda")
-        p = st["params"].to(F64).view(out // 16, -1, 2, 8, 2)
+        p = st["params"].to(F64).transpose(1, 2).reshape(out // 16, 2, 8, -1, 2)
         for j in range(4):
             for n in range(4):
                 c = _word_codes(words[..., j, n], [0, 4, 1, 5, 2, 6, 3, 7]).permute(0, 2, 3, 1, 4)
                 at = torch.arange(words.shape[1], device="cuda") * 128 + 32 * n + 8 * j
-                s = p[:, at // group].permute(0, 2, 3, 1, 4)
+                s = p[:, :, :, at // group]
                 w[..., at[:, None] + torch.arange(8, device="cuda")] = c * s[..., 0, None] + s[..., 1, None]
         y = st["x"].to(F64) @ w.view(out, -1)[:, :inn].T
         y = y + st["bias"].to(F64) if st["bias"] is not None else y
