@@ -221,6 +221,31 @@ int et_1x16_prefer_dense(int in, int out, int nvec);
 int et_1x16_densify(const int32_t* tile_idx, const int32_t* row_idx, const et_half* data, int nvec,
                     int in, int out, et_half* dense, et_stream stream);
 
+/* 4-bit weights with group scales.  Every `group` (32, 64 or 128) consecutive input features of an output row
+ * share one fp16 pair (s, m); a weight is c * s + m with a code c = 0 .. 15, quantised as the cache of
+ * et_kv4_write_fwd is (see there).  Arrays, nb = ceil(in / 128):
+ *     codes   bytes [out/16][nb][2][32][16]: half h, lane 4 i + j of block b of panel p holds row
+ *             16 p + 8 h + i, as four 32-bit words n with features 128 b + 32 n + 8 j + f, f < 8,
+ *             feature f in nibble (f >> 1) + 4 (f & 1);
+ *     params  fp16  [out/16][nb][16][128 / group][2]: (s, m) of the row's groups in the block.
+ *   Features past `in` have code 0 and do not count in their group; groups past it have s = m = 0.
+ *   et_w4_sizes   bytes of the two arrays;
+ *   et_w4_pack    quantises a dense W[out, in] (device) into them;
+ *   et_w4_densify dense[out, in] = fp16(c s + m), limited to +-65504, for et_linear_dense_fwd;
+ *   et_linear_w4_fwd  the forward pass.  Few tokens: codes and fp16 activations are multiplied as they are,
+ *     scales applied to fp32 sums (one pass over the 4-bit weights, no rounding of a weight); many tokens:
+ *     the weights are expanded to fp16 operand tiles in shared memory in front of the tcgen05 product.
+ *     An activation that is not finite leaves every output of its token without a finite value.
+ * codes, params, X, Y 16-byte aligned (bias: 2); in and out multiples of 16.  Like every weight, codes and
+ * params must be complete (stream synchronised) before the first Linear call that uses them.  Stands beside
+ * the weight formats of mat_type/; the reference has no quantised one. */
+int et_w4_sizes(int in, int out, int group, size_t* code_bytes, size_t* param_bytes);
+int et_w4_pack(const et_half* W, int in, int out, int group, uint8_t* codes, et_half* params, et_stream stream);
+int et_w4_densify(const uint8_t* codes, const et_half* params, int in, int out, int group, et_half* dense,
+                  et_stream stream);
+int et_linear_w4_fwd(const uint8_t* codes, const et_half* params, int group, const et_half* bias,
+                     const et_half* X, et_half* Y, int T, int in, int out, int act, et_stream stream);
+
 /* Host-side validators for index arrays that live in HOST memory (call before upload).
  * Return ET_OK or ET_ERR_INDEX; they never touch the GPU. */
 int et_validate_tile_mat(const int32_t* row_ptr, const int32_t* row_off, int nnz_tiles, int in,
@@ -364,6 +389,86 @@ int et_fused_vo_attention_pruned_fwd(const et_half* Q, const et_half* K, const e
                                      et_stream stream);
 
 /* =================================================================================
+ * Key/value cache in 4 bits, and attention over it
+ *
+ * The reference recomputes the whole sequence for every answer (Encoder/Encoder.h:81-96 keeps
+ * nothing between calls) and has no counterpart of these operators.
+ *
+ * Numbers: 32 consecutive features of a token and head form a group; its values are held as
+ * c * s + m with codes c = 0 .. 15 and one fp16 pair (s, m):
+ *     m = min, s = fp16(fp32(fp32(max - min) / 15)), c = round((x - m) / s) limited to 0 .. 15,
+ * the quotient rounded once, ties to even; s = 0 has c = 0.  A group that holds an infinity or
+ * NaN stores s = m = NaN.  |x - (c s + m)| is at most s / 2, but for the limit (s rounded down
+ * leaves the largest value up to s / 100 above 15 s + m).
+ *
+ * Pages: a sequence's tokens live in pages of `page` tokens, found through table[batch, table_ld]
+ * (int32 page numbers, position t in page table[b][t / page]); pages may be shared between
+ * sequences that only read them.  The four arrays, ng = ceil(max(dh_qk, dh_v) / 32):
+ *     k_codes, v_codes    bytes  [num_pages][nkv][page][16 * ng]
+ *     k_params, v_params  fp16   [num_pages][nkv][page][ng][2]       (s, m)
+ *   K row: 32-bit word j * ng + g (j < 4, g < ng) holds features 32 g + 8 j + f, f < 8, feature f
+ *          in nibble (f >> 1) + 4 (f & 1): nibbles 16 bits apart are neighbouring features.
+ *   V row: 16-bit unit i * ng + g (i < 8) holds features 32 g + 4 i + f, f < 4, in nibble f.
+ *   Features past the head's width have code 0 and do not count in their group; groups past it
+ *   have s = m = 0.
+ * page: a power of two, 16 or more.  dh_qk, dh_v: multiples of 16, at most 128.  All arrays
+ * 16-byte aligned.
+ *
+ * Page numbers and lengths live on the device and are checked there: a position past the table or
+ * a page number outside 0 .. num_pages - 1 is never followed; it is reported by et_device_error
+ * (601), a write to it is dropped, a read gives zeros (attention: a value of zero).
+ * ================================================================================= */
+typedef struct {
+    int num_pages, page, nkv, dh_qk, dh_v;
+    uint8_t* k_codes;
+    et_half* k_params;
+    uint8_t* v_codes;
+    et_half* v_params;
+} et_kv4_t;
+
+/* Bytes of one code array and of one parameter array (K and V have the same); the array pointers
+ * are not read. */
+int et_kv4_sizes(const et_kv4_t* cache, size_t* code_bytes, size_t* param_bytes);
+
+/* Quantises K[batch*seq, ldk] and V[batch*seq, ldv] (head h at feature h * dh) into the cache:
+ * row b * seq + i of sequence b goes to position start[b] + i, for i < new_len[b].  start NULL:
+ * 0; new_len NULL: seq.  Positions that several rows write hold one of them or a mixture. */
+int et_kv4_write_fwd(const et_kv4_t* cache, const et_half* K, const et_half* V, int ldk, int ldv,
+                     const int32_t* table, int table_ld, const int32_t* start,
+                     const int32_t* new_len, int batch, int seq, et_stream stream);
+
+/* Reads positions start[b] .. start[b] + len[b] of every sequence back into rows b * seq + i of
+ * K[batch*seq, ldk] and V[batch*seq, ldv] as fp16(c s + m), limited to +-65504.  Rows i >= len[b]
+ * are left as they were.  start NULL: 0; len NULL: seq. */
+int et_kv4_read_fwd(const et_kv4_t* cache, et_half* K, et_half* V, int ldk, int ldv,
+                    const int32_t* table, int table_ld, const int32_t* start, const int32_t* len,
+                    int batch, int seq, et_stream stream);
+
+/* Attention of new queries over the cache:
+ *   Z[b*seq+i, h*dh_v ..] = softmax_t( scale * Q_i.K_t + mask ) V_t over t < kv_len[b],
+ * nhead a multiple of cache->nkv (query head h reads key/value head h / (nhead / nkv)).
+ * kv_len[b] counts the cached tokens, the queries' own included (write them first).  q_len[b]
+ * rows of sequence b are queries (NULL: seq); the others leave their rows of Z as they were.
+ *   ET_MASK_NONE      every cached token is visible;
+ *   ET_MASK_CAUSAL    query i sees t <= kv_len[b] - q_len[b] + i: the queries are the newest tokens;
+ *   ET_MASK_ADDITIVE  fp16 mask[seq, ldm] added to the scaled scores, ldm >= max_len.
+ * A query that sees nothing (kv_len 0, or every score -inf) yields zeros.  What stands in a masked
+ * place, NaN included, does not reach the output.
+ * max_len: the largest kv_len (at most table_ld * page); longer sequences are cut there and
+ * reported (601).  Q.K is exact up to fp32 sums (codes and fp16 queries are multiplied as they
+ * are), probabilities enter the second product with 22 bits.
+ * The long axis is split over thread blocks when there are few rows; their fp32 partial results
+ * go to the workspace (et_attention_kv4_workspace_bytes; 0: none needed), which calls that may
+ * overlap on the GPU must not share.  Nothing of it has to be set or kept.  */
+size_t et_attention_kv4_workspace_bytes(const et_kv4_t* cache, int batch, int seq, int nhead,
+                                        int max_len);
+int et_attention_kv4_fwd(const et_kv4_t* cache, const et_half* Q, et_half* Z, const int32_t* table,
+                         int table_ld, const int32_t* kv_len, const int32_t* q_len, int batch,
+                         int seq, int nhead, int ldq, int ldz, int max_len, int mask_kind,
+                         const et_half* mask, int ldm, float scale, void* workspace,
+                         size_t workspace_bytes, et_stream stream);
+
+/* =================================================================================
  * Whole encoder layer (post-LN), the call Encoder<config>::forward makes
  * (Encoder/Encoder.h:81-96):
  *   a = O(attention(QKV(x)));  y = LN1(a + x);  out = LN2(W2 act(W1 y + b1) + b2 + y)
@@ -381,6 +486,7 @@ int et_fused_vo_attention_pruned_fwd(const et_half* Q, const et_half* K, const e
 #define ET_FMT_ROW 4         /* kept output rows (row_mat)                                 */
 #define ET_FMT_COL 5         /* kept input columns (col_mat)                               */
 #define ET_FMT_CSR 6         /* CSR                                                        */
+#define ET_FMT_W4 7          /* 4-bit codes with group scales (et_w4_pack)                 */
 
 /* One Linear layer of the encoder in any of the reference's weight formats.  The index and
  * count fields are shared between formats:
@@ -392,6 +498,7 @@ int et_fused_vo_attention_pruned_fwd(const et_half* Q, const et_half* K, const e
  *   ROW               rows[nn_row, in]       row_id[nn_row]   -              nn_row
  *   COL               cols[out, nn_col]      col_id[nn_col]   -              nn_col
  *   CSR               data[nnz]              indptr[out + 1]  indices[nnz]   nnz
+ *   W4                codes (bytes)          params           -              group size
  * (argument meaning as in the et_linear_*_fwd call of each format). */
 typedef struct {
     int format;             /* one of ET_FMT_*                                          */
@@ -421,6 +528,18 @@ int et_encoder_layer_fwd(const et_encoder_layer_t* layer, const et_half* x, et_h
                          int batch, int seq, int mask_kind, const et_half* mask,
                          const int32_t* valid_len, void* workspace, size_t workspace_bytes,
                          et_stream stream);
+
+/* The layer over `seq` NEW tokens of every sequence, the earlier ones in a 4-bit cache of this layer (one
+ * cache per layer; cache->nkv = nhead, head widths as the layer's): the new tokens' keys and values are
+ * written at start[b] .., then attended over causally (et_kv4_write_fwd, et_attention_kv4_fwd), and the rest of
+ * the layer follows.  kv_len[b] = start[b] + new_len[b]; new_len NULL: seq.  Rows i >= new_len[b] of `out` hold
+ * anything.  Every weight format serves; ET_FMT_W4 is the one made for few tokens. */
+size_t et_encoder_layer_cached_workspace_bytes(const et_encoder_layer_t* layer, const et_kv4_t* cache,
+                                               int batch, int seq, int max_len);
+int et_encoder_layer_cached_fwd(const et_encoder_layer_t* layer, const et_kv4_t* cache, const et_half* x,
+                                et_half* out, int batch, int seq, const int32_t* table, int table_ld,
+                                const int32_t* start, const int32_t* kv_len, const int32_t* new_len,
+                                int max_len, void* workspace, size_t workspace_bytes, et_stream stream);
 
 /* =================================================================================
  * Head-parallel form of the layer, for ONE long sequence spread over several GPUs (the

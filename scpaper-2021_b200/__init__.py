@@ -20,7 +20,7 @@ LIB_PATH = os.path.join(_HERE, "libet_b200_hooks.so" if os.environ.get("ET_B200_
 
 ACT_NONE, ACT_RELU, ACT_GELU = 0, 1, 2
 MASK_NONE, MASK_CAUSAL, MASK_PADDING, MASK_ADDITIVE = 0, 1, 2, 3
-FMT_DENSE, FMT_TILE, FMT_TILE_PACKED, FMT_1X16, FMT_ROW, FMT_COL, FMT_CSR = range(7)
+FMT_DENSE, FMT_TILE, FMT_TILE_PACKED, FMT_1X16, FMT_ROW, FMT_COL, FMT_CSR, FMT_W4 = range(8)
 
 # Every symbol include/et_b200.h declares (checked by the CPU test-suite against the header).
 ABI_SYMBOLS = [
@@ -40,6 +40,10 @@ ABI_SYMBOLS = [
     "et_fused_vo_attention_fwd", "et_linear_vo_fwd",
     "et_encoder_layer_workspace_bytes", "et_encoder_layer_fwd",
     "et_attention_units_fwd", "et_encoder_attention_units_fwd", "et_encoder_after_attention_fwd",
+    "et_w4_sizes", "et_w4_pack", "et_w4_densify", "et_linear_w4_fwd",
+    "et_kv4_sizes", "et_kv4_write_fwd", "et_kv4_read_fwd",
+    "et_attention_kv4_workspace_bytes", "et_attention_kv4_fwd",
+    "et_encoder_layer_cached_workspace_bytes", "et_encoder_layer_cached_fwd",
 ]
 
 
@@ -62,6 +66,12 @@ class EncoderLayerDesc(ctypes.Structure):
                 ("vdim", c_int), ("ff", c_int), ("act", c_int)]
 
 
+class KV4Desc(ctypes.Structure):
+    """et_kv4_t"""
+    _fields_ = [("num_pages", c_int), ("page", c_int), ("nkv", c_int), ("dh_qk", c_int), ("dh_v", c_int),
+                ("k_codes", c_void_p), ("k_params", c_void_p), ("v_codes", c_void_p), ("v_params", c_void_p)]
+
+
 _lib = None
 
 
@@ -78,6 +88,10 @@ def lib() -> ctypes.CDLL:
         L.et_launch_count.restype = ctypes.c_longlong
         L.et_encoder_layer_workspace_bytes.restype = c_size_t
         L.et_encoder_layer_workspace_bytes.argtypes = [c_void_p, c_int, c_int]
+        L.et_attention_kv4_workspace_bytes.restype = c_size_t
+        L.et_attention_kv4_workspace_bytes.argtypes = [c_void_p, c_int, c_int, c_int, c_int]
+        L.et_encoder_layer_cached_workspace_bytes.restype = c_size_t
+        L.et_encoder_layer_cached_workspace_bytes.argtypes = [c_void_p, c_void_p, c_int, c_int, c_int]
         _lib = L
     return _lib
 
@@ -159,6 +173,13 @@ _SIGNATURES = {
     "et_fused_vo_attention_fwd": "ppppp" "iiiiiiii" "ppfp",
     "et_fused_vo_attention_pruned_fwd": "ppppippp" "iiiiiiii" "ppfp",
     "et_encoder_layer_fwd": "pppiii" "pppzp",
+    "et_w4_pack": "piiippp",
+    "et_w4_densify": "ppiiipp",
+    "et_linear_w4_fwd": "ppippp" "iiiip",
+    "et_kv4_write_fwd": "pppiipippiip",
+    "et_kv4_read_fwd": "pppiipippiip",
+    "et_attention_kv4_fwd": "ppppipp" "iiiiiii" "pifpzp",
+    "et_encoder_layer_cached_fwd": "ppppiipippp" "ipzp",
 }
 _KINDS = {"p": c_void_p, "i": c_int, "z": c_size_t, "f": c_float}
 _calls = {}
@@ -335,6 +356,90 @@ def linear_csr(x, indptr, indices, data, out, bias=None, act=ACT_NONE):
     return y
 
 
+def _require(name: str, dtype, *tensors) -> None:
+    """Tensors of a call: of one type, on the current device, with contiguous rows."""
+    dev = _torch_c()._cuda_getDevice()
+    for t in tensors:
+        if t is None:
+            continue
+        if t.dtype is not dtype:
+            raise EtError(f"{name}: a tensor is {t.dtype}, {dtype} is wanted")
+        if not t.is_cuda or t.device.index != dev:
+            raise EtError(f"{name}: a tensor is on {t.device}, the current device is cuda:{dev}")
+        if t.dim() and t.stride(-1) != 1 and t.shape[-1] != 1:
+            raise EtError(f"{name}: the values of a row must be contiguous")
+
+
+def _row_stride(t) -> int:
+    """Stride of a matrix's rows (a single row may report any)."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+class W4Weight:
+    """A Linear weight in 4 bits: codes and one fp16 (scale, minimum) pair per `group` input features of an output
+    row (32, 64 or 128), quantised on the GPU from a dense W[out, in].  from_arrays() takes the two arrays in
+    the layout that et_b200.h states instead."""
+
+    def __init__(self, w, group: int = 128):
+        import torch
+        _require("W4Weight", torch.float16, w)
+        if w.dim() != 2 or not w.is_contiguous():
+            raise EtError("W4Weight: a contiguous matrix [out, in] is wanted")
+        out, inn = w.shape
+        self._set(inn, out, group)
+        self.codes = torch.empty(self.code_shape, dtype=torch.uint8, device=w.device)
+        self.params = torch.empty(self.param_shape, dtype=torch.float16, device=w.device)
+        _call("et_w4_pack", _a(w), inn, out, group, _a(self.codes), _a(self.params), _raw_stream())
+        torch.cuda.current_stream().synchronize()  # weights must be complete before their first use
+
+    def _set(self, inn: int, out: int, group: int) -> None:
+        code_bytes, param_bytes = c_size_t(0), c_size_t(0)
+        check(lib().et_w4_sizes(c_int(inn), c_int(out), c_int(group), ctypes.byref(code_bytes),
+                                ctypes.byref(param_bytes)), "et_w4_sizes")
+        nb = (inn + 127) // 128
+        self.inn, self.out, self.group = inn, out, group
+        self.code_shape = (out // 16, nb, 2, 32, 16)
+        self.param_shape = (out // 16, nb, 16, 128 // group, 2)
+
+    @classmethod
+    def from_arrays(cls, codes, params, inn: int, out: int, group: int):
+        import torch
+        w = cls.__new__(cls)
+        w._set(inn, out, group)
+        _require("W4Weight", torch.uint8, codes)
+        _require("W4Weight", torch.float16, params)
+        if tuple(codes.shape) != w.code_shape or tuple(params.shape) != w.param_shape:
+            raise EtError(f"W4Weight: codes {w.code_shape} and params {w.param_shape} are wanted")
+        if not codes.is_contiguous() or not params.is_contiguous():
+            raise EtError("W4Weight: contiguous arrays are wanted")
+        w.codes, w.params = codes, params
+        return w
+
+    def densify(self):
+        """The dense fp16 [out, in] weight that the codes stand for."""
+        import torch
+        dense = torch.empty((self.out, self.inn), dtype=torch.float16, device=self.codes.device)
+        _call("et_w4_densify", _a(self.codes), _a(self.params), self.inn, self.out, self.group, _a(dense),
+              _raw_stream())
+        torch.cuda.current_stream().synchronize()  # weights must be complete before their first use
+        return dense
+
+
+def linear_w4(x, w: "W4Weight", bias=None, act=ACT_NONE, out=None):
+    """act(x W^T + bias) with a 4-bit weight; `out`: optional preallocated [T, out] result."""
+    import torch
+    T, inn = x.shape
+    if inn != w.inn or not x.is_contiguous():
+        raise EtError(f"linear_w4: contiguous activations [T, {w.inn}] are wanted")
+    y = _empty((T, w.out), x) if out is None else out
+    _require("linear_w4", torch.float16, x, bias, y)
+    if y.shape != (T, w.out) or not y.is_contiguous() or (bias is not None and bias.shape != (w.out,)):
+        raise EtError(f"linear_w4: out [{T}, {w.out}] and bias [{w.out}] are wanted")
+    _call("et_linear_w4_fwd", _a(w.codes), _a(w.params), w.group, _a(bias), _a(x), _a(y), T, inn, w.out, act,
+          _raw_stream())
+    return y
+
+
 # ---- normalisation / element-wise ---------------------------------------------------------
 
 def skip_layernorm(src, skip, gamma, beta, out=None):
@@ -447,6 +552,114 @@ def fused_vo_attention(q, k, vo, bias_o, batch, seq, nhead, dh_qk, emdim, mask_k
     return out
 
 
+class KV4Cache:
+    """A paged key/value cache in 4 bits (layout and numbers: et_kv4_t in et_b200.h).  Pages are named by a table,
+    int32 [batch, pages of a sequence], that the caller keeps: position t of sequence b lives in page
+    table[b, t // page].  All calls take it, so one cache serves changing batches."""
+
+    def __init__(self, num_pages: int, page: int, nkv: int, dh_qk: int, dh_v: int, device="cuda"):
+        import torch
+        self.desc = KV4Desc(num_pages=num_pages, page=page, nkv=nkv, dh_qk=dh_qk, dh_v=dh_v)
+        code_bytes, param_bytes = c_size_t(0), c_size_t(0)
+        check(lib().et_kv4_sizes(ctypes.byref(self.desc), ctypes.byref(code_bytes), ctypes.byref(param_bytes)),
+              "et_kv4_sizes")
+        self.num_pages, self.page, self.nkv, self.dh_qk, self.dh_v = num_pages, page, nkv, dh_qk, dh_v
+        ng = (max(dh_qk, dh_v) + 31) // 32
+        codes, params = (num_pages, nkv, page, 16 * ng), (num_pages, nkv, page, ng, 2)
+        self.k_codes = torch.zeros(codes, dtype=torch.uint8, device=device)
+        self.k_params = torch.zeros(params, dtype=torch.float16, device=device)
+        self.v_codes, self.v_params = torch.zeros_like(self.k_codes), torch.zeros_like(self.k_params)
+        for name in ("k_codes", "k_params", "v_codes", "v_params"):
+            setattr(self.desc, name, getattr(self, name).data_ptr())
+        self._at = ctypes.addressof(self.desc)
+        self._workspace_bytes = {}
+
+    def workspace_bytes(self, batch: int, seq: int, nhead: int, max_len: int) -> int:
+        """Scratch of attention_kv4 for these sizes."""
+        key = (batch, seq, nhead, max_len)
+        n = self._workspace_bytes.get(key)
+        if n is None:
+            n = self._workspace_bytes[key] = int(lib().et_attention_kv4_workspace_bytes(self._at, *key))
+        return n
+
+
+def _check_pages(name: str, cache: "KV4Cache", batch: int, table, *lengths) -> None:
+    import torch
+    _require(name, torch.int32, table, *lengths)
+    if cache.k_codes.device != table.device:
+        raise EtError(f"{name}: the cache is on {cache.k_codes.device}")
+    if table.dim() != 2 or table.shape[0] != batch:
+        raise EtError(f"{name}: a page table [{batch}, pages] is wanted")
+    for n in lengths:
+        if n is not None and n.shape != (batch,):
+            raise EtError(f"{name}: one length per sequence ({batch}) is wanted")
+
+
+def _check_rows(name: str, rows: int, **widths) -> None:
+    for what, (t, width) in widths.items():
+        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width:
+            raise EtError(f"{name}: {what} [{rows}, {width}] is wanted")
+
+
+def kv4_write(cache: "KV4Cache", k, v, table, start, batch: int, seq: int, new_len=None) -> None:
+    """Quantises k [batch * seq, nkv * dh_qk] and v (views of a fused projection serve) into positions
+    start[b] .. of every sequence; rows i >= new_len[b] are padding.  start None: 0."""
+    import torch
+    _require("kv4_write", torch.float16, k, v)
+    _check_pages("kv4_write", cache, batch, table, start, new_len)
+    _check_rows("kv4_write", batch * seq, k=(k, cache.nkv * cache.dh_qk), v=(v, cache.nkv * cache.dh_v))
+    _call("et_kv4_write_fwd", cache._at, _a(k), _a(v), _row_stride(k), _row_stride(v), _a(table),
+          _row_stride(table), _a(start), _a(new_len), batch, seq, _raw_stream())
+
+
+def kv4_read(cache: "KV4Cache", table, batch: int, seq: int, start=None, length=None, out=None):
+    """(k, v) in fp16 from positions start[b] .. start[b] + length[b] (seq where None) of every sequence;
+    rows behind a sequence's last are left as they were (`out`: a preallocated pair)."""
+    import torch
+    _check_pages("kv4_read", cache, batch, table, start, length)
+    rows = batch * seq
+    if out is None:
+        make = torch.empty if length is None else torch.zeros
+        out = tuple(make((rows, cache.nkv * d), dtype=torch.float16, device=table.device)
+                    for d in (cache.dh_qk, cache.dh_v))
+    k, v = out
+    _require("kv4_read", torch.float16, k, v)
+    _check_rows("kv4_read", rows, k=(k, cache.nkv * cache.dh_qk), v=(v, cache.nkv * cache.dh_v))
+    _call("et_kv4_read_fwd", cache._at, _a(k), _a(v), _row_stride(k), _row_stride(v), _a(table),
+          _row_stride(table), _a(start), _a(length), batch, seq, _raw_stream())
+    return k, v
+
+
+def attention_kv4(cache: "KV4Cache", q, table, kv_len, batch: int, seq: int, nhead: int, max_len=None,
+                  mask_kind=MASK_CAUSAL, mask=None, q_len=None, scale=None, out=None, workspace=None):
+    """softmax(q k^T * scale + mask) v of q [batch * seq, nhead * dh_qk] over the kv_len[b] cached tokens of every
+    sequence, the queries' own (its newest, written first) included.  max_len: the largest kv_len (the page
+    table's reach where None); a tight one lets the call split the sequence well.  q_len[b] < seq: padding rows,
+    left as they were.  mask: fp16 [seq, >= max_len] for MASK_ADDITIVE.  workspace: optional scratch of
+    cache.workspace_bytes(...) bytes, not shared with calls that may overlap."""
+    import torch
+    if max_len is None:
+        max_len = table.shape[1] * cache.page
+    z = out
+    if z is None:
+        z = (torch.empty if q_len is None else torch.zeros)(
+            (batch * seq, nhead * cache.dh_v), dtype=torch.float16, device=q.device)
+    _require("attention_kv4", torch.float16, q, z, mask)
+    _check_pages("attention_kv4", cache, batch, table, kv_len, q_len)
+    _check_rows("attention_kv4", batch * seq, q=(q, nhead * cache.dh_qk), out=(z, nhead * cache.dh_v))
+    if mask is not None and (mask.dim() != 2 or mask.shape[0] < seq):
+        raise EtError(f"attention_kv4: a mask [{seq}, {max_len}] is wanted")
+    if workspace is None:
+        n = cache.workspace_bytes(batch, seq, nhead, max_len)
+        workspace = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+    _call("et_attention_kv4_fwd", cache._at, _a(q), _a(z), _a(table), _row_stride(table), _a(kv_len), _a(q_len),
+          batch, seq, nhead, _row_stride(q), _row_stride(z), max_len, mask_kind, _a(mask),
+          0 if mask is None else (_row_stride(mask) if mask.shape[1] >= max_len else mask.shape[1]),
+          (1.0 / cache.dh_qk ** 0.5) if scale is None else scale,
+          _a(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(), _raw_stream())
+    return z
+
+
 # ---- encoder layer / stack ----------------------------------------------------------------
 
 def linear_vo_pruned(x, w_vo_c, bias, batch, seq, nhead, emdim):
@@ -481,7 +694,7 @@ class EncoderLayer:
     `formats` overrides that per weight ("wqkv", "wo", "w1", "w2"): "dense", "1x16" (the vector
     kernel), "1x16_auto" (et_1x16_prefer_dense chooses between it and the dense GEMM on the
     expanded weight), "csr", ("row", ids) (kept output rows) or ("col", ids) (kept input
-    columns).  ("row", ids) on "w1" with ("col", ids) on "w2" over the same `ids` array object
+    columns), "w4" or ("w4", group) (4-bit codes with group scales).  ("row", ids) on "w1" with ("col", ids) on "w2" over the same `ids` array object
     describes pruned hidden units of the feed-forward block: both products run at the kept
     width."""
 
@@ -535,6 +748,11 @@ class EncoderLayer:
                     _, cols = synth.dense_to_col(W, np.asarray(ids))
                     d.format, d.nnz_tiles = FMT_COL, int(len(ids))
                     d.row_ptr, d.weight = dev_ids(ids).data_ptr(), dev(cols).data_ptr()
+                elif kind == "w4":
+                    w4 = W4Weight(dev(W), 128 if isinstance(fmt, str) else fmt[1])
+                    self._keep[-1] = w4  # (the dense weight is not kept)
+                    d.format, d.nnz_tiles = FMT_W4, w4.group
+                    d.weight, d.row_ptr = w4.codes.data_ptr(), w4.params.data_ptr()
                 elif kind == "csr":
                     indptr, indices, data = synth.dense_to_csr(W)
                     d.format, d.nnz_tiles = FMT_CSR, int(indices.shape[0])
@@ -603,6 +821,25 @@ class EncoderLayer:
                 valid_len=None):
         _call("et_encoder_layer_fwd", ctypes.byref(self.desc), _a(x), _a(out), batch, seq,
               mask_kind, _a(mask), _a(valid_len), _a(workspace),
+              workspace.numel() * workspace.element_size(), _raw_stream())
+        return out
+
+    def cached_workspace_bytes(self, cache: "KV4Cache", batch: int, seq: int, max_len: int) -> int:
+        return int(lib().et_encoder_layer_cached_workspace_bytes(ctypes.addressof(self.desc), cache._at, batch, seq,
+                                                                 max_len))
+
+    def forward_cached(self, x, out, cache: "KV4Cache", table, start, kv_len, batch, seq, max_len, workspace,
+                       new_len=None):
+        """The layer over `seq` new tokens of every sequence at positions start[b] .., the earlier ones in
+        `cache` (this layer's own); kv_len = start + new_len."""
+        import torch
+        _require("forward_cached", torch.float16, x, out)
+        _check_pages("forward_cached", cache, batch, table, start, kv_len, new_len)
+        _check_rows("forward_cached", batch * seq, x=(x, self.hidden), out=(out, self.hidden))
+        if not x.is_contiguous() or not out.is_contiguous():
+            raise EtError("forward_cached: contiguous x and out are wanted")
+        _call("et_encoder_layer_cached_fwd", ctypes.addressof(self.desc), cache._at, _a(x), _a(out), batch, seq,
+              _a(table), _row_stride(table), _a(start), _a(kv_len), _a(new_len), max_len, _a(workspace),
               workspace.numel() * workspace.element_size(), _raw_stream())
         return out
 
@@ -981,6 +1218,63 @@ class EncoderStack:
             done.record(self.streams[g - 1])
             main.wait_event(done)
         return self.buf[(len(self.layers) - 1) & 1]
+
+
+class CachedStack:
+    """N chained encoder layers (causal) that keep what they have seen: every layer has a 4-bit key/value cache
+    for `batch` sequences of up to `max_len` tokens.  forward() takes the next tokens of all sequences - a whole
+    prompt, then one token at a time - and returns their outputs; reset() starts over.  Lengths live on the
+    device, so a captured forward() can be replayed for token after token (the caller then counts them: a token
+    past max_len is dropped and reported by device_error() as 601)."""
+
+    def __init__(self, layers, batch: int, max_len: int, page: int = 64, device="cuda"):
+        import torch
+        self.layers = list(layers)
+        self.batch = batch
+        per = (max_len + page - 1) // page
+        self.max_len = max_len
+        self.caches = []
+        for l in self.layers:
+            d = l.desc
+            self.caches.append(KV4Cache(batch * per, page, d.nhead, d.kdim // d.nhead, d.vdim // d.nhead, device))
+        self.table = torch.arange(batch * per, dtype=torch.int32, device=device).view(batch, per)
+        self.start = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.kv_len = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.used = 0  # the most that any sequence may hold, counted on the host
+        self._buffers = {}  # tokens per sequence -> workspace and two activation buffers
+
+    def reset(self) -> None:
+        self.kv_len.zero_()
+        self.used = 0
+
+    def _buffers_of(self, seq: int):
+        import torch
+        got = self._buffers.get(seq)
+        if got is None:
+            ws = max(l.cached_workspace_bytes(c, self.batch, seq, self.max_len)
+                     for l, c in zip(self.layers, self.caches))
+            if ws == 0:
+                raise EtError("invalid encoder layer description")
+            dev = self.table.device
+            got = self._buffers[seq] = (torch.empty(ws, dtype=torch.uint8, device=dev), [
+                torch.empty((self.batch * seq, self.layers[0].hidden), dtype=torch.float16, device=dev)
+                for _ in range(2)])
+        return got
+
+    def forward(self, x, seq: int, new_len=None):
+        """x [batch * seq, hidden]: `seq` new tokens of every sequence, of which new_len[b] (int32) count.  The
+        result is overwritten by the next call with the same `seq`."""
+        if self.used + seq > self.max_len:
+            raise EtError(f"CachedStack: {self.used} + {seq} tokens do not fit into {self.max_len}")
+        ws, buf = self._buffers_of(seq)
+        self.start.copy_(self.kv_len)
+        self.kv_len.add_(seq if new_len is None else new_len)
+        cur = x
+        for i, (layer, cache) in enumerate(zip(self.layers, self.caches)):
+            cur = layer.forward_cached(cur, buf[i & 1], cache, self.table, self.start, self.kv_len, self.batch, seq,
+                                       self.max_len, ws, new_len)
+        self.used += seq
+        return cur
 
 
 class HostPipeline:

@@ -13,6 +13,7 @@
 
 #include "common.cuh"
 #include "kernels.h"
+#include "kv4.h"
 
 namespace et {
 namespace {
@@ -176,6 +177,10 @@ int run_linear(const et_linear_t& lin, const __half* X, __half* Y, int T, int ac
         case ET_FMT_1X16:
             return et_linear_1x16_fwd(lin.row_ptr, lin.row_off, lin.weight, lin.nnz_tiles, lin.bias,
                                       Xe, Ye, T, lin.in, lin.out, act, stream);
+        case ET_FMT_W4:
+            return et_linear_w4_fwd(reinterpret_cast<const uint8_t*>(lin.weight),
+                                    reinterpret_cast<const et_half*>(lin.row_ptr), lin.nnz_tiles, lin.bias,
+                                    Xe, Ye, T, lin.in, lin.out, act, stream);
         case ET_FMT_ROW:
             return et_linear_row_fwd(lin.row_ptr, lin.weight, lin.nnz_tiles, lin.bias, Xe, Ye, T,
                                      lin.in, lin.out, act, stream);
@@ -306,6 +311,56 @@ int ffn_block(const et_encoder_layer_t* layer, const LayerBuffers& b, int T, __h
                                      reinterpret_cast<__half*>(out), T, layer->hidden, s);
 }
 
+// b.z (the attention's output) -> y = LN1(O(z) + x) -> out = LN2(FFN(y) + y)
+int after_attention(const et_encoder_layer_t* layer, const LayerBuffers& b, const __half* xin, int T, __half* out,
+                    cudaStream_t s) {
+    int st;
+    const __half* wo = reinterpret_cast<const __half*>(layer->o.weight);
+    const __half* bo = reinterpret_cast<const __half*>(layer->o.bias);
+    const __half* g1 = reinterpret_cast<const __half*>(layer->ln1_gamma);
+    const __half* e1 = reinterpret_cast<const __half*>(layer->ln1_beta);
+    const NarrowPlan narrow = layer->o.format == ET_FMT_DENSE &&
+                                          narrow_takes(b.z, layer->vdim, wo, bo, xin, g1, e1, b.y)
+                                      ? pick_narrow_ln(T, layer->hidden, layer->vdim)
+                                      : NarrowPlan{0, 0};
+    if (narrow.splits > 0) {
+        if ((st = narrow_linear_ln(narrow, b.z, layer->vdim, wo, bo, xin, g1, e1, b.y, b.part, T,
+                                       layer->hidden, s)) != ET_OK)
+            return st;
+    } else if (layer->o.format == ET_FMT_DENSE && ln_fused(1, T, layer->hidden, layer->vdim) &&
+               gemm_ln_applies(T, layer->hidden, layer->vdim)) {
+        // O projection, residual and LayerNorm in one kernel
+        if ((st = launch_gemm_ln(b.z, layer->vdim,
+                                     reinterpret_cast<const __half*>(layer->o.weight), layer->vdim,
+                                     reinterpret_cast<const __half*>(layer->o.bias), xin,
+                                     layer->hidden,
+                                     reinterpret_cast<const __half*>(layer->ln1_gamma),
+                                     reinterpret_cast<const __half*>(layer->ln1_beta), b.y,
+                                     layer->hidden, T, layer->hidden, layer->vdim, s)) != ET_OK)
+            return st;
+    } else {
+        if ((st = run_linear(layer->o, b.z, b.a, T, ET_ACT_NONE, b, s)) != ET_OK) return st;
+        if ((st = launch_skip_layernorm(b.a, xin,
+                                            reinterpret_cast<const __half*>(layer->ln1_gamma),
+                                            reinterpret_cast<const __half*>(layer->ln1_beta), b.y,
+                                            T, layer->hidden, s)) != ET_OK)
+            return st;
+    }
+    return ffn_block(layer, b, T, out, s);
+}
+
+// Layer and cache describe the same heads.
+int check_cached(const et_encoder_layer_t* L, const et_kv4_t* c) {
+    const int st = check_layer(L);
+    if (st != ET_OK) return st;
+    if (!c) return ET_ERR_INVALID_ARG;
+    Kv4View v;
+    const int cst = kv4_view(c, v, false);
+    if (cst != ET_OK) return cst;
+    if (c->nkv != L->nhead || c->dh_qk != L->kdim / L->nhead || c->dh_v != L->vdim / L->nhead) return ET_ERR_SHAPE;
+    return ET_OK;
+}
+
 }  // namespace
 }  // namespace et
 
@@ -371,38 +426,50 @@ int et_encoder_layer_fwd(const et_encoder_layer_t* layer, const et_half* x, et_h
             ET_OK)
             return st;
     }
-    const __half* wo = reinterpret_cast<const __half*>(layer->o.weight);
-    const __half* bo = reinterpret_cast<const __half*>(layer->o.bias);
-    const __half* g1 = reinterpret_cast<const __half*>(layer->ln1_gamma);
-    const __half* e1 = reinterpret_cast<const __half*>(layer->ln1_beta);
-    const et::NarrowPlan narrow = layer->o.format == ET_FMT_DENSE &&
-                                          et::narrow_takes(b.z, layer->vdim, wo, bo, xin, g1, e1, b.y)
-                                      ? et::pick_narrow_ln(T, layer->hidden, layer->vdim)
-                                      : et::NarrowPlan{0, 0};
-    if (narrow.splits > 0) {
-        if ((st = et::narrow_linear_ln(narrow, b.z, layer->vdim, wo, bo, xin, g1, e1, b.y, b.part, T,
-                                       layer->hidden, s)) != ET_OK)
-            return st;
-    } else if (layer->o.format == ET_FMT_DENSE && et::ln_fused(1, T, layer->hidden, layer->vdim) &&
-               et::gemm_ln_applies(T, layer->hidden, layer->vdim)) {
-        // O projection, residual and LayerNorm in one kernel
-        if ((st = et::launch_gemm_ln(b.z, layer->vdim,
-                                     reinterpret_cast<const __half*>(layer->o.weight), layer->vdim,
-                                     reinterpret_cast<const __half*>(layer->o.bias), xin,
-                                     layer->hidden,
-                                     reinterpret_cast<const __half*>(layer->ln1_gamma),
-                                     reinterpret_cast<const __half*>(layer->ln1_beta), b.y,
-                                     layer->hidden, T, layer->hidden, layer->vdim, s)) != ET_OK)
-            return st;
-    } else {
-        if ((st = et::run_linear(layer->o, b.z, b.a, T, ET_ACT_NONE, b, s)) != ET_OK) return st;
-        if ((st = et::launch_skip_layernorm(b.a, xin,
-                                            reinterpret_cast<const __half*>(layer->ln1_gamma),
-                                            reinterpret_cast<const __half*>(layer->ln1_beta), b.y,
-                                            T, layer->hidden, s)) != ET_OK)
-            return st;
-    }
-    return et::ffn_block(layer, b, T, reinterpret_cast<__half*>(out), s);
+    return et::after_attention(layer, b, xin, T, reinterpret_cast<__half*>(out), s);
+}
+
+// ---- the layer over new tokens of sequences whose earlier tokens are in a 4-bit cache --------
+size_t et_encoder_layer_cached_workspace_bytes(const et_encoder_layer_t* layer, const et_kv4_t* cache, int batch,
+                                               int seq, int max_len) {
+    if (et::check_cached(layer, cache) != ET_OK || batch <= 0 || seq <= 0 || max_len <= 0) return 0;
+    return et::carve(layer, batch, seq, nullptr).total +
+           et::align256(et_attention_kv4_workspace_bytes(cache, batch, seq, layer->nhead, max_len));
+}
+
+int et_encoder_layer_cached_fwd(const et_encoder_layer_t* layer, const et_kv4_t* cache, const et_half* x,
+                                et_half* out, int batch, int seq, const int32_t* table, int table_ld,
+                                const int32_t* start, const int32_t* kv_len, const int32_t* new_len, int max_len,
+                                void* workspace, size_t workspace_bytes, et_stream stream) {
+    int st = et::check_cached(layer, cache);
+    if (st != ET_OK) return st;
+    et::Kv4View v;  // everything is checked before the first launch
+    if ((st = et::kv4_view(cache, v, true)) != ET_OK) return st;
+    if (!x || !out || !table || !start || !kv_len || batch <= 0 || seq <= 0 || max_len <= 0 || table_ld <= 0)
+        return ET_ERR_INVALID_ARG;
+    if (static_cast<int64_t>(table_ld) << v.page_shift < max_len) return ET_ERR_SHAPE;
+    if ((st = et::kv4_check_attention(v, batch, seq, layer->nhead, max_len)) != ET_OK) return st;
+    if (!workspace) return ET_ERR_WORKSPACE;
+    if (reinterpret_cast<uintptr_t>(workspace) & 255u) return ET_ERR_ALIGNMENT;
+    if (!et::aligned16(x) || !et::aligned16(out)) return ET_ERR_ALIGNMENT;
+    const et::LayerBuffers b = et::carve(layer, batch, seq, workspace);
+    const size_t att = et_attention_kv4_workspace_bytes(cache, batch, seq, layer->nhead, max_len);
+    if (workspace_bytes < b.total + et::align256(att)) return ET_ERR_WORKSPACE;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int T = batch * seq;
+    const __half* xin = reinterpret_cast<const __half*>(x);
+    const int ldqkv = 2 * layer->kdim + layer->vdim;
+    if ((st = et::run_linear(layer->qkv, xin, b.qkv, T, ET_ACT_NONE, b, s)) != ET_OK) return st;
+    const et_half* qkv = reinterpret_cast<const et_half*>(b.qkv);
+    if ((st = et_kv4_write_fwd(cache, qkv + layer->kdim, qkv + 2 * layer->kdim, ldqkv, ldqkv, table, table_ld, start,
+                               new_len, batch, seq, stream)) != ET_OK)
+        return st;
+    if ((st = et_attention_kv4_fwd(cache, qkv, reinterpret_cast<et_half*>(b.z), table, table_ld, kv_len, new_len,
+                                   batch, seq, layer->nhead, ldqkv, layer->vdim, max_len, ET_MASK_CAUSAL, nullptr, 0,
+                                   1.0f / sqrtf(static_cast<float>(layer->kdim / layer->nhead)),
+                                   static_cast<uint8_t*>(workspace) + b.total, att, stream)) != ET_OK)
+        return st;
+    return et::after_attention(layer, b, xin, T, reinterpret_cast<__half*>(out), s);
 }
 
 // ---- head-parallel form: the layer in two halves around the ranks' one exchange step --------

@@ -94,6 +94,11 @@ int launch_linear_expand_packed(const uint32_t* pk_mask, const int* pk_off, cons
                                 const __half* bias, const __half* X, __half* Y, int T, int in, int out,
                                 int act, cudaStream_t stream);
 
+// The Linear over 4-bit weights (et_linear_w4_fwd) for many tokens, expanded the same way; see
+// linear_expand.cu.  Arguments already checked.
+int launch_linear_expand_w4(const uint8_t* codes, const __half* params, int group, const __half* bias,
+                            const __half* X, __half* Y, int T, int in, int out, int act, cudaStream_t stream);
+
 // Fused attention (see attention.cu).  row_per_thread = false keeps every head width on the kernel whose
 // body attention_fuse_o.cu shares, so that the two give the same bits.
 int launch_attention(const __half* Q, const __half* K, const __half* V, __half* Z, int batch,

@@ -1,5 +1,5 @@
 // Linear layers over irregular weight formats on the tensor cores:
-//     Y[T, out] = act(X[T, in] . W^T + bias),   W stored as 1x16 vectors, packed 16x16 tiles or CSR.
+//     Y[T, out] = act(X[T, in] . W^T + bias),   W stored as 1x16 vectors, packed 16x16 tiles, CSR or 4-bit codes.
 //
 // The tensor core cannot skip single vectors or values, but expanding them is cheap next to
 // multiplying: a CTA owns BN output features and MB blocks of 128 tokens, and eight warps write the
@@ -20,13 +20,14 @@
 #include "common.cuh"
 #include "gemm_common.cuh"
 #include "kernels.h"
+#include "quant4.cuh"
 
 namespace et {
 namespace {
 
 using namespace gemm;
 
-enum : int { FMT_VEC = 0, FMT_PACKED = 1, FMT_CSRM = 2 };
+enum : int { FMT_VEC = 0, FMT_PACKED = 1, FMT_CSRM = 2, FMT_QUANT = 3 };
 
 constexpr int X_MAX_A = 8;                       // activation stages at most
 constexpr int X_MAX_B = 4;                       // weight buffers at most
@@ -38,7 +39,8 @@ constexpr int X_EXP_THREADS = 32 * X_EXP_WARPS;
 constexpr int X_ROW_LIST = 128 + 1;
 
 struct ExpandArgs {
-    // 1x16: tile_idx / row_idx / data; packed: masks / offsets / tiles; CSR: indptr / indices / data
+    // 1x16: tile_idx / row_idx / data; packed: masks / offsets / tiles; CSR: indptr / indices / data;
+    // 4 bits: params / - / codes
     const int* idx0;
     const int* idx1;
     const __half* data;
@@ -46,6 +48,7 @@ struct ExpandArgs {
     const __half* X;
     __half* Y;
     int T, in, out, act;
+    int group;      // 4 bits: features per (s, m)
     int mb;         // token blocks per CTA
     int ckb, nbuf;  // K blocks per weight buffer, weight buffers
     int na;         // activation stages
@@ -172,6 +175,64 @@ struct PackedExpander {
         o_next = o_next2;
         index_of(kb + 3 * step, m_next2, o_next2);
         fetch(m, o);
+    }
+};
+
+// The same for 4-bit codes: every element of the 16 rows is written.  A code becomes fp16 exactly (1024 + c,
+// less 1024), and c s + m is rounded to fp16 once: the tensor core cannot scale its sums per group, so the
+// operand has to carry the scale.  Lane 4 i + j expands words 2 q and 2 q + 1 (q: which half of the 128-feature
+// block) of rows i and i + 8, fetched one block ahead.
+struct QuantExpander {
+    const uint2* codes;
+    const uint32_t* params;
+    int nb, nkb, gb, lane;
+    uint2 v[2];
+    uint32_t sm[2][2];  // [row half][word]
+
+    __device__ __forceinline__ void fetch(int kb) {
+        if (kb >= nkb) return;
+        const int b = kb >> 1, q = kb & 1;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            v[h] = __ldg(codes + ((static_cast<size_t>(b) * 2 + h) * 32 + lane) * 2 + q);
+            const uint32_t* p = params + (static_cast<size_t>(b) * 16 + 8 * h + (lane >> 2)) * gb;
+            sm[h][0] = __ldg(p + ((2 * q) * gb >> 2));
+            sm[h][1] = __ldg(p + ((2 * q + 1) * gb >> 2));
+        }
+    }
+    __device__ __forceinline__ void init(const ExpandArgs& a, int panel, int lane_) {
+        lane = lane_;
+        nb = (a.in + 127) >> 7;
+        nkb = (a.in + BK - 1) / BK;
+        gb = 128 / a.group;
+        codes = reinterpret_cast<const uint2*>(a.data) + static_cast<size_t>(panel) * nb * 128;
+        params = reinterpret_cast<const uint32_t*>(a.idx0) + static_cast<size_t>(panel) * nb * 16 * gb;
+    }
+    __device__ __forceinline__ void start(int kb, int) { fetch(kb); }
+    __device__ __forceinline__ void write(uint8_t* tile, int kb, int step) {
+        if (kb >= nkb) return;
+        const __half2 base = __floats2half2_rn(1024.f, 1024.f);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int row = 8 * h + (lane >> 2), j = lane & 3;
+            uint8_t* line = tile + row * 128;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const uint32_t w = n ? v[h].y : v[h].x;
+                const __half2 pair = *reinterpret_cast<const __half2*>(&sm[h][n]);
+                const __half2 s = __low2half2(pair), m = __high2half2(pair);
+                uint32_t o[4];
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    const uint32_t c = ((w >> (4 * p)) & q4::NIBBLES) | 0x64006400u;
+                    const __half2 y = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), base), s, m);
+                    o[p] = *reinterpret_cast<const uint32_t*>(&y);
+                }
+                *reinterpret_cast<uint4*>(line + (((n * 4 + j) ^ (row & 7)) * 16)) =
+                    make_uint4(o[0], o[1], o[2], o[3]);
+            }
+        }
+        fetch(kb + step);
     }
 };
 
@@ -420,7 +481,9 @@ linear_expand_kernel(const __grid_constant__ CUtensorMap tmX, const ExpandArgs g
             constexpr int SETS = BN / 16;
             const int set = w % SETS, sub = w / SETS;  // sub < ckb
             const bool live = n0 + set * 16 < g.out;
-            typename std::conditional<FMT == FMT_VEC, VecExpander, PackedExpander>::type x;
+            typename std::conditional<
+                FMT == FMT_QUANT, QuantExpander,
+                typename std::conditional<FMT == FMT_VEC, VecExpander, PackedExpander>::type>::type x;
             if (live) {
                 x.init(g, (n0 >> 4) + set, lane);
                 x.start(sub, g.ckb);
@@ -433,10 +496,12 @@ linear_expand_kernel(const __grid_constant__ CUtensorMap tmX, const ExpandArgs g
                     ok = __all_sync(0xffffffffu, ok);
                 }
                 uint8_t* tile = sB + buf * buf_bytes + sub * (BN * 128) + set * (16 * 128);
+                if (FMT != FMT_QUANT) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    reinterpret_cast<uint4*>(tile)[i * 32 + lane] = make_uint4(0u, 0u, 0u, 0u);
-                __syncwarp();
+                    for (int i = 0; i < 4; ++i)
+                        reinterpret_cast<uint4*>(tile)[i * 32 + lane] = make_uint4(0u, 0u, 0u, 0u);
+                    __syncwarp();
+                }
                 if (live) x.write(tile, c * g.ckb + sub, g.ckb);
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -507,7 +572,7 @@ linear_expand_kernel(const __grid_constant__ CUtensorMap tmX, const ExpandArgs g
             // twice, and whatever is not finite.  (An activation that is not finite leaves no element of its
             // row finite, so one of 32 tells.  A pass of its own: inside the loop above it cost 3 % of
             // 1024 -> 3072 at 3072 tokens.)
-            if (any_dup || __any_sync(0xffffffffu, odd))
+            if (FMT != FMT_QUANT && (any_dup || __any_sync(0xffffffffu, odd)))
                 for (int u = half; u < mb * NG; u += 2) {
                     const int tb = u / NG, cg = u - tb * NG;
                     const int row0 = m0 + tb * BM + q * 32, m = row0 + lane;
@@ -669,6 +734,22 @@ int launch_linear_expand_packed(const uint32_t* pk_mask, const int* pk_off, cons
     a.out = out;
     a.act = act;
     return launch_expand<FMT_PACKED>(a, stream);
+}
+
+int launch_linear_expand_w4(const uint8_t* codes, const __half* params, int group, const __half* bias,
+                            const __half* X, __half* Y, int T, int in, int out, int act, cudaStream_t stream) {
+    ExpandArgs a = {};
+    a.idx0 = reinterpret_cast<const int*>(params);
+    a.data = reinterpret_cast<const __half*>(codes);
+    a.group = group;
+    a.bias = bias;
+    a.X = X;
+    a.Y = Y;
+    a.T = T;
+    a.in = in;
+    a.out = out;
+    a.act = act;
+    return launch_expand<FMT_QUANT>(a, stream);
 }
 
 }  // namespace et
