@@ -6,22 +6,25 @@
 // so the tensor core multiplies fp16 queries by codes (exact; fp32 sums) and scale and minimum are applied to
 // its results.  For the second product the scale goes to the probability instead,
 //     out[d in g] = ( sum_t (p_t s_g(t)) (c_t[d] - 8)  +  sum_t p_t (m_g(t) + 8 s_g(t)) ) / sum_t p_t,
-// with p s split into two fp16 numbers (22 bits) that share the fragment of one product: rows 0-7 of the
-// 16-row operand hold the high parts, rows 8-15 the low ones (up to eight query rows), or two products (16).
-// (Codes less 8: sums of codes of one sign grow with the sequence while the output shrinks, and the tensor core
-// cuts its fp32 sums: at 32768 tokens that cost half of the result's own rounding again, 3.2e-4 for 2.1e-4.)
-// The softmax is online; its reference is the running maximum of the scaled scores plus the exponent of the
-// running largest s, so that p s <= 1 whatever the magnitude of V.
+// with p s split into two fp16 numbers (22 bits) and one product for each.  (Codes less 8: sums of codes of one
+// sign grow with the sequence while the output shrinks, and the tensor core cuts its fp32 sums: at 32768 tokens
+// that cost half of the result's own rounding again, 3.2e-4 for 2.1e-4.)  The softmax is online; its reference is
+// the running maximum of the scaled scores plus the exponent of the running largest s, so that p s < 1 whatever
+// the magnitude of V.
 //
-// A thread block owns up to 16 query rows that share a key/value head (the heads of a group times the query tokens) and a
-// chunk of the sequence; its four warps take 32-token tiles in turn, each with a ring of asynchronous copies of its
-// own (page contents land in shared memory as they are; no thread waits for another warp in the loop).  With
-// few rows the sequence is split over blocks whose partial results a second kernel joins.
+// A thread block owns up to 16 query rows that share a key/value head (the heads of a group times the query
+// tokens) and a chunk of the sequence; its four warps take 32-token tiles in turn, each with a ring of bulk copies
+// of its own (page contents land in shared memory as they are; no thread waits for another warp in the
+// loop).  With few rows the sequence is split over blocks whose partial results a second kernel joins.
 //
-// Layout of a tile in registers (lane = 4 i + j): the cache stores rows so that a lane's words are consecutive.  K:
-// lane (i, j) holds word j of every group of token tau(i) = (i >> 1) + 4 (i & 1), which makes its score columns
-// 2 j, 2 j + 1 tokens j and j + 4; V: unit i of every group of tokens j, j + 4, j + 8, j + 12 - the order in which those scores
-// sit in the second product's operand.
+// Layout.  Both products have the cache as their 16-row operand and eight query rows as their 8-column one: a few
+// rows then waste little of the tensor core and of the registers (with the rows on the 16 side, half
+// empty, the accumulators took 64 registers a thread instead of 32 at 128 features, and spilled).  Lane 4 i + j holds
+// word j of every group of token tau(i) = (i >> 1) + 4 (i & 1) of K, and unit i of every group of tokens j, j + 4,
+// j + 8, j + 12 of V: the order in which the transposed probabilities (movmatrix) lie along the second product.
+//
+// What bounds it: instruction issue.  Unpacking alone takes 1.25 instructions per element and lane (a shift and
+// an AND for two codes, a subtraction for V's), scales and the softmax as much again.
 #include "kernels.h"
 #include "kv4.h"
 #include "quant4.cuh"
@@ -31,7 +34,6 @@ namespace {
 
 constexpr int TILE = 32;      // tokens of a warp's tile
 constexpr int WARPS = 4;
-constexpr int STAGES = 4;
 constexpr int THREADS = 32 * WARPS;
 constexpr int MAX_SPLITS = 64;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -52,16 +54,6 @@ struct AttArgs {
     float scale_log2;
     int* err_word;
 };
-
-__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool valid) {
-    const int n = valid ? 16 : 0;  // 0: zeros are written, nothing is read
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 
 // NG 32-bit words at p (shared memory, 4 NG-byte aligned)
 template <int NG>
@@ -97,24 +89,51 @@ __device__ __forceinline__ void lds_units(const uint8_t* p, uint32_t (&u)[(NG + 
 
 template <int NG>
 struct Smem {
+    static constexpr int STAGES = NG == 4 ? 2 : 3;
     static constexpr int CODES = TILE * 16 * NG, PARAMS = TILE * 4 * NG;
     static constexpr int STAGE = 2 * (CODES + PARAMS);  // K codes, V codes, K params, V params
     static constexpr int RING = STAGES * STAGE;
-    static constexpr int WIDE = TILE * NG * 16;  // (s, m) of K and of V as fp32
+    static constexpr int WIDE = TILE * NG * 16;  // (s, s, m, m) of K, then of V, as fp32
     static constexpr int WARP = RING + WIDE;
-    static constexpr int TOTAL = WARPS * WARP;
+    static constexpr int BARS = WARPS * WARP;
+    static constexpr int TOTAL = BARS + WARPS * STAGES * 8 + 16;
 };
 
-// RT: 8-row tiles (1: the 16-row operand's other half carries the low parts; 2: 16 query rows).
-template <int NG, int RT>
-__global__ void __launch_bounds__(THREADS, NG <= 2 ? 4 : (NG == 3 ? 3 : 2)) attention_kv4_kernel(const AttArgs a) {
+// Thread blocks that share an SM, by registers (and, at two stages of the widest rows, shared memory).
+constexpr int blocks_per_sm(int ng, int nt) { return nt == 1 ? (ng <= 2 ? 5 : 4) : (ng <= 2 ? 4 : 3); }
+
+// Place of (s, s, m, m) of group g and token t: eight lanes that read eight tokens meet no bank conflict.
+template <int NG>
+__device__ __forceinline__ int wide_at(int t, int g) {
+    return NG == 4 ? t * 4 + (g ^ ((t >> 1) & 3)) : NG == 2 ? t * 2 + (g ^ ((t >> 2) & 1)) : t * NG + g;
+}
+
+// Transposes an 8 x 8 matrix of fp16: lane 4 i + j holds row i, columns 2 j and 2 j + 1, before and after.
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+// NT: tiles of eight query rows.
+template <int NG, int NT>
+__global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_kernel(const AttArgs a) {
     using S = Smem<NG>;
-    constexpr int D = 32 * NG;
-    extern __shared__ __align__(16) uint8_t smem[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int D = 32 * NG, STAGES = S::STAGES;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int warp = uniform_warp_id(), lane = threadIdx.x & 31;
     const int i = lane >> 2, j = lane & 3;
+    const int tau = (i >> 1) + 4 * (i & 1);
     uint8_t* ring = smem + warp * S::WARP;
-    float4* wide = reinterpret_cast<float4*>(ring + S::RING);  // [token][group] sK, mK, sV, mV + 8 sV
+    float4* wide = reinterpret_cast<float4*>(ring + S::RING);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BARS) + warp * STAGES;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::BARS + WARPS * STAGES * 8);
+    if (lane == 0) {
+        for (int k = 0; k < STAGES; ++k) mbar_init(&bars[k], 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    __syncthreads();
 
     pdl_wait();
     pdl_launch_dependents();
@@ -132,39 +151,11 @@ __global__ void __launch_bounds__(THREADS, NG <= 2 ? 4 : (NG == 3 ? 3 : 2)) atte
     nq = nq < 0 ? 0 : (nq > a.seq ? a.seq : nq);
 
     // ---- rows: row r of the tile is query token r / ratio, head kvh * ratio + r % ratio
-    const int row0 = rt * 8 * RT;
+    const int row0 = rt * 8 * NT;
     if (row0 >= nq * a.ratio) return;  // (rows are ordered by query token)
-    int limit[RT];                     // tokens that a row sees
-    uint32_t qf[NG][RT][4];            // its queries: features 32 g + 8 j .. + 8
-    float qs[NG][RT];                  // sum of the group's queries times 2^-24 (the codes carry that factor)
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const int r = row0 + 8 * t + i;
-        const int qi = r / a.ratio, head = kvh * a.ratio + r % a.ratio;
-        const bool live = qi < nq;
-        // (rows that are not there compute on zero queries and are never stored)
-        limit[t] = !live ? (a.mask_kind == ET_MASK_ADDITIVE ? 0 : INT32_MAX)
-                         : (a.mask_kind == ET_MASK_CAUSAL ? len - nq + qi + 1 : len);
-        const __half* q = a.Q + (static_cast<int64_t>(b) * a.seq + qi) * a.ldq + head * a.c.dh[0] + 8 * j;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (live && 32 * g + 8 * j < a.c.dh[0]) v = __ldcg(reinterpret_cast<const uint4*>(q + 32 * g));
-            qf[g][t][0] = v.x, qf[g][t][1] = v.y, qf[g][t][2] = v.z, qf[g][t][3] = v.w;
-            float sum = 0.f;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qf[g][t][k]));
-                sum += f.x + f.y;
-            }
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            qs[g][t] = sum * 0x1p-24f;
-        }
-    }
-    int most, least;  // the largest and smallest limit: those of the last and first row
+    int most, least;  // the largest and smallest number of tokens that a row sees: the last and first row's
     {
-        const int last = (row0 + 8 * RT < nq * a.ratio ? row0 + 8 * RT : nq * a.ratio) - 1;
+        const int last = (row0 + 8 * NT < nq * a.ratio ? row0 + 8 * NT : nq * a.ratio) - 1;
         if (a.mask_kind == ET_MASK_CAUSAL) {
             least = len - nq + row0 / a.ratio + 1;
             most = len - nq + last / a.ratio + 1;
@@ -173,13 +164,13 @@ __global__ void __launch_bounds__(THREADS, NG <= 2 ? 4 : (NG == 3 ? 3 : 2)) atte
         }
         most = most < 0 ? 0 : most;
     }
-    // this block's chunk of the sequence, and the warp's tiles in it
+    // this block's chunk of the sequence, and the warp's tiles in it: warp, warp + 4, ...
     const int per = ((most + a.splits - 1) / a.splits + TILE - 1) / TILE * TILE;
     const int64_t first64 = static_cast<int64_t>(split) * per;
     const int first = first64 < most ? static_cast<int>(first64) : most;
     const int end = first + per < most ? first + per : most;
     const int ntile = (end - first + TILE - 1) / TILE;
-    const int mine = ntile > warp ? (ntile - warp + WARPS - 1) / WARPS : 0;  // tiles warp, warp + 4, ...
+    const int mine = ntile > warp ? (ntile - warp + WARPS - 1) / WARPS : 0;
 
     // ---- page numbers of 16 tiles at a time, one half tile (16 tokens) to a lane
     const int* table = a.table + static_cast<int64_t>(b) * a.table_ld;
@@ -191,197 +182,261 @@ __global__ void __launch_bounds__(THREADS, NG <= 2 ? 4 : (NG == 3 ? 3 : 2)) atte
         return id;
     };
     int pages = page_of(0), pages_next = page_of(16);
-    // copies tile n of this warp (call with n = 0, 1, 2, ... in order)
+    // Copies of tile n of this warp (called with n = 0, 1, 2, ... in order): lanes 0 .. 7 fetch half tile
+    // `lane & 1` of one of the four arrays each.
+    const int kind = (lane >> 1) & 3;  // K codes, V codes, K params, V params
+    const uint8_t* src = kind < 2 ? a.c.codes[kind] : reinterpret_cast<const uint8_t*>(a.c.params[kind & 1]);
+    const int row_bytes = kind < 2 ? 16 * NG : 4 * NG;
+    const int dst = (kind < 2 ? kind * S::CODES : 2 * S::CODES + (kind & 1) * S::PARAMS) + (lane & 1) * 16 * row_bytes;
+    uint32_t there = 0;  // two bits per issued tile, the newest lowest: which halves were fetched
     auto issue = [&](int n) {
-        if (n < mine) {
-            if (n != 0 && (n & 15) == 0) {
-                pages = pages_next;
-                pages_next = page_of(n + 16);
-            }
-            uint8_t* st = ring + (n % STAGES) * S::STAGE;
-            const int pos = first + (n * WARPS + warp) * TILE;
-            const int id0 = __shfl_sync(0xffffffffu, pages, (n & 15) * 2);
-            const int id1 = __shfl_sync(0xffffffffu, pages, (n & 15) * 2 + 1);
-            // rows of the two half tiles (of 0 where nothing is read: any address inside the arrays will do)
-            const int64_t r0 = id0 < 0 ? 0 : kv4_row(a.c, id0, pos, kvh);
-            const int64_t r1 = id1 < 0 ? 0 : kv4_row(a.c, id1, pos + 16, kvh);
-#pragma unroll
-            for (int of = 0; of < 2; ++of) {
-#pragma unroll
-                for (int u = 0; u < NG; ++u) {  // 32 NG pieces of codes, half of them per half tile
-                    const int p = u * 32 + lane;
-                    const bool hi = p >= 16 * NG;
-                    const int id = hi ? id1 : id0;
-                    const uint8_t* src = a.c.codes[of] + (hi ? r1 : r0) * (16 * NG) + (hi ? p - 16 * NG : p) * 16;
-                    cp_async16(st + of * S::CODES + p * 16, id < 0 ? a.c.codes[of] : src, id >= 0);
-                }
-                // 8 NG pieces of parameters
-                if (lane < 8 * NG) {
-                    const bool hi = lane >= 4 * NG;
-                    const int id = hi ? id1 : id0;
-                    const uint8_t* base = reinterpret_cast<const uint8_t*>(a.c.params[of]);
-                    const uint8_t* src = base + (hi ? r1 : r0) * (4 * NG) + (hi ? lane - 4 * NG : lane) * 16;
-                    cp_async16(st + 2 * S::CODES + of * S::PARAMS + lane * 16, id < 0 ? base : src, id >= 0);
-                }
-            }
+        there <<= 2;
+        if (n >= mine) return;
+        if (n != 0 && (n & 15) == 0) {
+            pages = pages_next;
+            pages_next = page_of(n + 16);
         }
-        cp_async_commit();  // (an empty group past the last tile, so that the count stays)
+        const int id = __shfl_sync(0xffffffffu, pages, (n & 15) * 2 + (lane & 1));
+        const uint32_t have = __ballot_sync(0xffffffffu, id >= 0) & 3u;
+        there |= have;
+        uint64_t* bar = &bars[n % STAGES];
+        if (lane == 0) mbar_arrive_expect_tx(bar, __popc(have) * (S::STAGE / 2));
+        __syncwarp();
+        if (lane < 8 && id >= 0) {
+            const int64_t row = kv4_row(a.c, id, first + (n * WARPS + warp) * TILE + (lane & 1) * 16, kvh);
+            bulk_load(ring + (n % STAGES) * S::STAGE + dst, src + row * row_bytes, 16 * row_bytes, bar);
+        }
     };
-
-    float acc[NG][4][4];  // [group][f]: the second product's fragments
-    float pm[NG][RT], l[RT], top[RT];
-    float e = -24.f;  // exponent: every s so far is <= 2^e
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-#pragma unroll
-        for (int f = 0; f < 4; ++f)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) acc[g][f][k] = 0.f;
-#pragma unroll
-        for (int t = 0; t < RT; ++t) pm[g][t] = 0.f;
-    }
-#pragma unroll
-    for (int t = 0; t < RT; ++t) l[t] = 0.f, top[t] = -INFINITY;
-
 #pragma unroll
     for (int n = 0; n < STAGES - 1; ++n) issue(n);
 
+    // ---- the rows' queries
+    int limit[NT][2];        // tokens that rows 8 t + 2 j, 8 t + 2 j + 1 see
+    uint32_t qf[NG][NT][4];  // row 8 t + i: features 32 g + 8 j .. + 8
+    uint64_t qs[NG][NT];     // rows 8 t + 2 j, + 1: sums over the group times 2^-24 (the codes carry that factor)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int r = row0 + 8 * t + i;
+        const int qi = r / a.ratio, head = kvh * a.ratio + r % a.ratio;
+        const __half* q = a.Q + (static_cast<int64_t>(b) * a.seq + qi) * a.ldq + head * a.c.dh[0] + 8 * j;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (qi < nq && 32 * g + 8 * j < a.c.dh[0]) v = __ldcg(reinterpret_cast<const uint4*>(q + 32 * g));
+            qf[g][t][0] = v.x, qf[g][t][1] = v.y, qf[g][t][2] = v.z, qf[g][t][3] = v.w;
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qf[g][t][k]));
+                sum += f.x + f.y;
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            sum *= 0x1p-24f;
+            const float s0 = __shfl_sync(0xffffffffu, sum, 8 * j), s1 = __shfl_sync(0xffffffffu, sum, 8 * j + 4);
+            qs[g][t] = pack_f32x2(s0, s1);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int qr = (row0 + 8 * t + 2 * j + h) / a.ratio;
+            // (rows that are not there compute on zero queries and are never stored)
+            limit[t][h] = qr >= nq ? (a.mask_kind == ET_MASK_ADDITIVE ? 0 : INT32_MAX)
+                                   : (a.mask_kind == ET_MASK_CAUSAL ? len - nq + qr + 1 : len);
+        }
+    }
+
+    float acc[NG][2][NT][4];  // [group][u]: features f = 2 u (elements 0, 1) and, times 16, 2 u + 1 (2, 3)
+    uint64_t pm[NG][NT];      // sums of p (m + 8 s), two rows
+    float l[NT][2], top[NT][2];
+    float e = -14.f;  // exponent: every s so far is < 2^e
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            pm[g][t] = 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc[g][k >> 2][t][k & 3] = 0.f;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) l[t][h] = 0.f, top[t][h] = -INFINITY;
+    }
+
+    const uint64_t minus_one = pack_f32x2(-1.f, -1.f);
+    bool ok = true;
     for (int n = 0; n < mine; ++n) {
-        cp_async_wait<STAGES - 2>();
+        if (!mbar_wait_bounded_warp(&bars[n % STAGES], (n / STAGES) & 1, abort_flag)) {
+            // (copies still in flight must land before the block's shared memory is given up)
+            for (int k = n; k < mine && k < n + STAGES - 1; ++k)
+                for (uint32_t it = 0; it < ET_SPIN_LIMIT && !mbar_try_wait(&bars[k % STAGES], (k / STAGES) & 1); ++it) {
+                }
+            if (lane == 0) report_error(a.err_word, abort_flag, DEV_TIMEOUT_KV4);
+            ok = false;
+            break;
+        }
         __syncwarp();
         issue(n + STAGES - 1);  // into the slot that the previous tile left
         const uint8_t* st = ring + (n % STAGES) * S::STAGE;
         const int tok0 = first + (n * WARPS + warp) * TILE;
+        // token `lane` counts: others (past the end, or of a page that is not there) are taken as zeros
+        const bool in = tok0 + lane < end && ((there >> (2 * (STAGES - 1) + (lane >> 4))) & 1u);
 
-        // ---- (s, m) of token `lane` to fp32; tokens past the end count as zeros
+        // ---- K's (s, m) to fp32; V's largest s, and whether all of V's are finite
+        uint32_t vp[NG];
         bool odd = false;
         uint32_t s_top = 0;
+        lds_words<NG>(st + 2 * S::CODES + S::PARAMS + lane * 4 * NG, vp);
         {
-            uint32_t kp[NG], vp[NG];
+            uint32_t kp[NG];
             lds_words<NG>(st + 2 * S::CODES + lane * 4 * NG, kp);
-            lds_words<NG>(st + 2 * S::CODES + S::PARAMS + lane * 4 * NG, vp);
-            const bool in = tok0 + lane < end;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const float2 k = __half22float2(*reinterpret_cast<const __half2*>(&kp[g]));
-                const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&vp[g]));
-                const bool fine = q4::finite16(vp[g]) && q4::finite16(vp[g] >> 16);
-                odd = odd || (in && !fine);
-                const uint32_t bits = in && fine ? __float_as_uint(fabsf(v.x)) : 0u;
-                s_top = bits > s_top ? bits : s_top;
-                wide[lane * NG + g] =
-                    in ? make_float4(k.x, k.y, v.x, fmaf(8.f, v.x, v.y)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                if (!in) kp[g] = vp[g] = 0u;
+                const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&kp[g]));
+                wide[wide_at<NG>(lane, g)] = make_float4(x.x, x.x, x.y, x.y);
+                if (!q4::finite16(vp[g]) || !q4::finite16(vp[g] >> 16)) {
+                    odd = true;
+                    vp[g] = 0u;
+                }
+                s_top = max(s_top, vp[g] & 0x7fffu);
             }
         }
         odd = __any_sync(0xffffffffu, odd);
         s_top = __reduce_max_sync(0xffffffffu, s_top);
-        // 2^(exponent + 1) >= s
-        const float e_new = fmaxf(e, static_cast<float>(static_cast<int>(s_top >> 23) - 126));
+        const float e_new = fmaxf(e, static_cast<float>(static_cast<int>(s_top >> 10) - 14));
         __syncwarp();
 
-        // ---- scores
-        float x[2][RT][4];  // [16-token block][row][token j, j + 4, j + 8, j + 12 of the block]
+        // ---- scores (times 2^-24): [16-token block][token tau, tau + 8][row 2 j, 2 j + 1]
+        float x[2][NT][2][2];
 #pragma unroll
-        for (int bk = 0; bk < 2; ++bk)
+        for (int bk = 0; bk < 2; ++bk) {
+            uint32_t k0[NG], k1[NG];
+            lds_words<NG>(st + (16 * bk + tau) * (16 * NG) + j * (4 * NG), k0);
+            lds_words<NG>(st + (16 * bk + tau + 8) * (16 * NG) + j * (4 * NG), k1);
+            uint64_t sum[NT][2];
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
-                const int base = 16 * bk + 8 * nt;
-                uint32_t kw[NG];
-                lds_words<NG>(st + (base + (i >> 1) + 4 * (i & 1)) * (16 * NG) + j * (4 * NG), kw);
-                float s0[RT], s1[RT];
+            for (int t = 0; t < NT; ++t) sum[t][0] = sum[t][1] = 0;
 #pragma unroll
-                for (int t = 0; t < RT; ++t) s0[t] = s1[t] = 0.f;
+            for (int g = 0; g < NG; ++g) {
+                uint32_t a0[4], a1[4];
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    float d[4];
-                    q4::mma0(d, qf[g][0][0], RT > 1 ? qf[g][RT - 1][0] : 0u, qf[g][0][1],
-                             RT > 1 ? qf[g][RT - 1][1] : 0u, kw[g] & q4::NIBBLES, (kw[g] >> 4) & q4::NIBBLES);
-                    q4::mma(d, qf[g][0][2], RT > 1 ? qf[g][RT - 1][2] : 0u, qf[g][0][3],
-                            RT > 1 ? qf[g][RT - 1][3] : 0u, (kw[g] >> 8) & q4::NIBBLES, (kw[g] >> 12) & q4::NIBBLES);
-                    const float2 p0 = *reinterpret_cast<const float2*>(&wide[(base + j) * NG + g]);
-                    const float2 p1 = *reinterpret_cast<const float2*>(&wide[(base + j + 4) * NG + g]);
-#pragma unroll
-                    for (int t = 0; t < RT; ++t) {
-                        s0[t] = fmaf(d[2 * t], p0.x, fmaf(qs[g][t], p0.y, s0[t]));
-                        s1[t] = fmaf(d[2 * t + 1], p1.x, fmaf(qs[g][t], p1.y, s1[t]));
-                    }
+                for (int p = 0; p < 4; ++p) {
+                    a0[p] = (k0[g] >> (4 * p)) & q4::NIBBLES;
+                    a1[p] = (k1[g] >> (4 * p)) & q4::NIBBLES;
                 }
+                const float4 m0 = wide[wide_at<NG>(16 * bk + tau, g)];
+                const float4 m1 = wide[wide_at<NG>(16 * bk + tau + 8, g)];
 #pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    x[bk][t][2 * nt] = s0[t] * a.scale_log2;
-                    x[bk][t][2 * nt + 1] = s1[t] * a.scale_log2;
+                for (int t = 0; t < NT; ++t) {
+                    float d[4];
+                    q4::mma0(d, a0[0], a1[0], a0[1], a1[1], qf[g][t][0], qf[g][t][1]);
+                    q4::mma(d, a0[2], a1[2], a0[3], a1[3], qf[g][t][2], qf[g][t][3]);
+                    sum[t][0] = fma_f32x2(pack_f32x2(d[0], d[1]), pack_f32x2(m0.x, m0.y),
+                                          fma_f32x2(qs[g][t], pack_f32x2(m0.z, m0.w), sum[t][0]));
+                    sum[t][1] = fma_f32x2(pack_f32x2(d[2], d[3]), pack_f32x2(m1.x, m1.y),
+                                          fma_f32x2(qs[g][t], pack_f32x2(m1.z, m1.w), sum[t][1]));
                 }
             }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                unpack_f32x2(sum[t][0], x[bk][t][0][0], x[bk][t][0][1]);
+                unpack_f32x2(sum[t][1], x[bk][t][1][0], x[bk][t][1][1]);
+            }
+        }
         if (tok0 + TILE > least || a.mask_kind == ET_MASK_ADDITIVE) {
+            const float per_unit = LOG2E / a.scale_log2;
 #pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                const int r = row0 + 8 * t + i;
-                const __half* mrow = a.mask + static_cast<int64_t>(r / a.ratio) * a.ldm;
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int bk = 0; bk < 2; ++bk)
+                for (int h = 0; h < 2; ++h) {
+                    const __half* mrow =
+                        a.mask + static_cast<int64_t>((row0 + 8 * t + 2 * j + h) / a.ratio) * a.ldm;
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int tok = tok0 + 16 * bk + j + 4 * u;
-                        if (tok >= limit[t]) x[bk][t][u] = -INFINITY;
+                    for (int k = 0; k < 4; ++k) {
+                        const int tok = tok0 + 8 * k + tau;
+                        float& v = x[k >> 1][t][k & 1][h];
+                        if (tok >= limit[t][h]) v = -INFINITY;
                         else if (a.mask_kind == ET_MASK_ADDITIVE) {
                             const float m = __half2float(__ldcg(mrow + tok));
-                            // (-inf hides the key whatever its score)
-                            x[bk][t][u] = m == -INFINITY ? -INFINITY : fmaf(m, LOG2E, x[bk][t][u]);
+                            v = m == -INFINITY ? -INFINITY : fmaf(m, per_unit, v);  // (-inf hides any score)
                         }
                     }
-            }
+                }
         }
 
         // ---- online softmax
-        float ref[RT];
         bool moved = false;
-        float scale_old[RT];
+        float ref[NT][2], shrink[NT][2];
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            float mx = -INFINITY;
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int bk = 0; bk < 2; ++bk)
-#pragma unroll
-                for (int u = 0; u < 4; ++u) mx = fmaxf(mx, x[bk][t][u]);
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            mx = fmaxf(mx, top[t]);
-            // a row that has seen nothing yet keeps sums of zero, whatever its reference
-            const float now = mx == -INFINITY ? 0.f : mx;
-            scale_old[t] = top[t] == -INFINITY ? 1.f : exp2f(top[t] - now + e - e_new);
-            moved = moved || scale_old[t] != 1.f;
-            top[t] = mx;
-            ref[t] = now + e_new;
-        }
+            for (int h = 0; h < 2; ++h) {
+                float mx = fmaxf(fmaxf(x[0][t][0][h], x[0][t][1][h]), fmaxf(x[1][t][0][h], x[1][t][1][h]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                mx = fmaxf(mx * a.scale_log2, top[t][h]);
+                // a row that has seen nothing yet keeps sums of zero, whatever its reference
+                const float now = mx == -INFINITY ? 0.f : mx;
+                shrink[t][h] = top[t][h] == -INFINITY ? 1.f : exp2f(top[t][h] - now + e - e_new);
+                moved = moved || shrink[t][h] != 1.f;
+                top[t][h] = mx;
+                ref[t][h] = now + e_new;
+            }
         e = e_new;
         if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                l[t] *= scale_old[t];
+            for (int t = 0; t < NT; ++t) {
+                l[t][0] *= shrink[t][0];
+                l[t][1] *= shrink[t][1];
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    pm[g][t] *= scale_old[t];
+                    pm[g][t] = mul_f32x2(pm[g][t], pack_f32x2(shrink[t][0], shrink[t][1]));
 #pragma unroll
-                    for (int f = 0; f < 4; ++f) {
-                        acc[g][f][2 * t] *= scale_old[t];
-                        acc[g][f][2 * t + 1] *= scale_old[t];
-                        if (RT == 1) {
-                            acc[g][f][2] *= scale_old[t];
-                            acc[g][f][3] *= scale_old[t];
-                        }
-                    }
+                    for (int k = 0; k < 8; ++k) acc[g][k >> 2][t][k & 3] *= shrink[t][k & 1];
                 }
             }
         }
 #pragma unroll
-        for (int bk = 0; bk < 2; ++bk)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int t = 0; t < RT; ++t)
+            for (int k = 0; k < 4; ++k)
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    x[bk][t][u] = exp2_approx(x[bk][t][u] - ref[t]);
-                    l[t] += x[bk][t][u];
+                for (int h = 0; h < 2; ++h) {
+                    float& v = x[k >> 1][t][k & 1][h];
+                    v = exp2_approx(fmaf(v, a.scale_log2, -ref[t][h]));
+                    l[t][h] += v;
                 }
+        if (odd) {  // a group of V that is not finite: NaN for the rows that see it, and for no other
+            const uint32_t* raw = reinterpret_cast<const uint32_t*>(st + 2 * S::CODES + S::PARAMS);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int tok = 8 * k + tau;
+                if (tok0 + tok >= end || !((there >> (2 * (STAGES - 1) + (tok >> 4))) & 1u)) continue;
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const uint32_t w = raw[tok * NG + g];
+                    if (q4::finite16(w) && q4::finite16(w >> 16)) continue;
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        float p0, p1;
+                        unpack_f32x2(pm[g][t], p0, p1);
+                        if (x[k >> 1][t][k & 1][0] != 0.f) p0 = NAN;
+                        if (x[k >> 1][t][k & 1][1] != 0.f) p1 = NAN;
+                        pm[g][t] = pack_f32x2(p0, p1);
+                    }
+                }
+            }
+        }
+
+        // ---- V's (s, m + 8 s) to fp32, in K's place
+        __syncwarp();
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&vp[g]));
+            const float m = fmaf(8.f, v.x, v.y);
+            wide[wide_at<NG>(lane, g)] = make_float4(v.x, v.x, m, m);
+        }
+        __syncwarp();
 
         // ---- second product
 #pragma unroll
@@ -392,79 +447,76 @@ __global__ void __launch_bounds__(THREADS, NG <= 2 ? 4 : (NG == 3 ? 3 : 2)) atte
                 lds_units<NG>(st + S::CODES + (16 * bk + j + 4 * u) * (16 * NG) + i * (2 * NG), vu[u]);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                uint32_t hi[RT][2], lo[RT][2];
-                float2 sm[4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    sm[u] = *(reinterpret_cast<const float2*>(&wide[(16 * bk + j + 4 * u) * NG + g]) + 1);
-#pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    float ps[4];
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const float p = x[bk][t][u];
-                        ps[u] = p * sm[u].x;
-                        float add = p * sm[u].y;
-                        if (odd && p == 0.f) ps[u] = add = 0.f;  // a hidden key's NaN stays hidden
-                        pm[g][t] += add;
-                    }
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        hi[t][h] = pack_half2(ps[2 * h], ps[2 * h + 1]);
-                        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[t][h]));
-                        lo[t][h] = pack_half2(ps[2 * h] - back.x, ps[2 * h + 1] - back.y);
-                    }
-                }
                 const uint32_t sel = g & 1 ? 0x7632u : 0x5410u;
                 const uint32_t w0 = __byte_perm(vu[0][g / 2], vu[1][g / 2], sel);
                 const uint32_t w1 = __byte_perm(vu[2][g / 2], vu[3][g / 2], sel);
+                const uint32_t w0h = w0 >> 8, w1h = w1 >> 8;
+                const uint32_t f0 = q4::centred(w0), f1 = q4::centred16(w0), f2 = q4::centred(w0h),
+                               f3 = q4::centred16(w0h);
+                const uint32_t g0 = q4::centred(w1), g1 = q4::centred16(w1), g2 = q4::centred(w1h),
+                               g3 = q4::centred16(w1h);
+                const float4 m0 = wide[wide_at<NG>(16 * bk + tau, g)];
+                const float4 m1 = wide[wide_at<NG>(16 * bk + tau + 8, g)];
 #pragma unroll
-                for (int f = 0; f < 4; ++f) {
-                    const uint32_t b0 = q4::centred(w0 >> (4 * f)), b1 = q4::centred(w1 >> (4 * f));
-                    if (RT == 1) {
-                        q4::mma(acc[g][f], hi[0][0], lo[0][0], hi[0][1], lo[0][1], b0, b1);
-                    } else {
-                        q4::mma(acc[g][f], hi[0][0], hi[RT - 1][0], hi[0][1], hi[RT - 1][1], b0, b1);
-                        q4::mma(acc[g][f], lo[0][0], lo[RT - 1][0], lo[0][1], lo[RT - 1][1], b0, b1);
+                for (int t = 0; t < NT; ++t) {
+                    uint32_t hi[2], lo[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float4& m = h ? m1 : m0;
+                        const uint64_t p = pack_f32x2(x[bk][t][h][0], x[bk][t][h][1]);
+                        const uint64_t ps = mul_f32x2(p, pack_f32x2(m.x, m.y));
+                        pm[g][t] = fma_f32x2(p, pack_f32x2(m.z, m.w), pm[g][t]);
+                        float p0, p1;
+                        unpack_f32x2(ps, p0, p1);
+                        const uint32_t top16 = pack_half2(p0, p1);
+                        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&top16));
+                        unpack_f32x2(fma_f32x2(pack_f32x2(back.x, back.y), minus_one, ps), p0, p1);
+                        hi[h] = transposed(top16);
+                        lo[h] = transposed(pack_half2(p0, p1));
                     }
+                    q4::mma(acc[g][0][t], f0, f1, g0, g1, hi[0], hi[1]);
+                    q4::mma(acc[g][1][t], f2, f3, g2, g3, hi[0], hi[1]);
+                    q4::mma(acc[g][0][t], f0, f1, g0, g1, lo[0], lo[1]);
+                    q4::mma(acc[g][1][t], f2, f3, g2, g3, lo[0], lo[1]);
                 }
             }
         }
     }
-    cp_async_wait<0>();
-    __syncthreads();  // every warp is done with its ring: it becomes the exchange area
+    if (!__syncthreads_and(ok)) return;  // every warp is done with its ring: it becomes the exchange area
 
     // ---- join the warps: [warp][row][D] sums and [warp][row][2] (reference, sum of p)
     float* xs = reinterpret_cast<float*>(smem);
-    constexpr int ROWS = 8 * RT;
-    static_assert(WARPS * ROWS * (D + 2) * 4 <= S::TOTAL, "exchange area");
+    constexpr int ROWS = 8 * NT;
+    static_assert(WARPS * ROWS * (D + 2) * 4 <= S::BARS, "exchange area");
     float* xml = xs + WARPS * ROWS * D;
+    auto over_tokens = [](float v) {
+        v += __shfl_xor_sync(0xffffffffu, v, 4);
+        v += __shfl_xor_sync(0xffffffffu, v, 8);
+        return v + __shfl_xor_sync(0xffffffffu, v, 16);
+    };
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        l[t] += __shfl_xor_sync(0xffffffffu, l[t], 1);
-        l[t] += __shfl_xor_sync(0xffffffffu, l[t], 2);
-        const int row = warp * ROWS + 8 * t + i;
-        if (j == 0) {
-            // (a row whose every score is NaN has no maximum, but is not empty)
-            xml[2 * row] = l[t] != l[t] && top[t] == -INFINITY ? 0.f : top[t] + e;
-            xml[2 * row + 1] = l[t];
+    for (int t = 0; t < NT; ++t) {
+        const int row = warp * ROWS + 8 * t + 2 * j;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            l[t][h] = over_tokens(l[t][h]);
+            if (i == 0) {
+                // (a row whose every score is NaN has no maximum, but is not empty)
+                xml[2 * (row + h)] = l[t][h] != l[t][h] && top[t][h] == -INFINITY ? 0.f : top[t][h] + e;
+                xml[2 * (row + h) + 1] = l[t][h];
+            }
         }
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-            float m = pm[g][t];
-            m += __shfl_xor_sync(0xffffffffu, m, 1);
-            m += __shfl_xor_sync(0xffffffffu, m, 2);
-            float o[2][4];
+            float m[2];
+            unpack_f32x2(pm[g][t], m[0], m[1]);
 #pragma unroll
-            for (int f = 0; f < 4; ++f)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float v = RT == 1 ? acc[g][f][h] + acc[g][f][2 + h] : acc[g][f][2 * t + h];
-                    o[h][f] = v + m;
-                }
-            float4* p = reinterpret_cast<float4*>(xs + row * D + 32 * g + 8 * j);
-            p[0] = make_float4(o[0][0], o[0][1], o[0][2], o[0][3]);
-            p[1] = make_float4(o[1][0], o[1][1], o[1][2], o[1][3]);
+            for (int h = 0; h < 2; ++h) {
+                m[h] = over_tokens(m[h]);
+                *reinterpret_cast<float4*>(xs + (row + h) * D + 32 * g + 4 * i) =
+                    make_float4(acc[g][0][t][h] + m[h], fmaf(acc[g][0][t][2 + h], 0.0625f, m[h]),
+                                acc[g][1][t][h] + m[h], fmaf(acc[g][1][t][2 + h], 0.0625f, m[h]));
+            }
         }
     }
     __syncthreads();
@@ -555,34 +607,36 @@ __global__ void __launch_bounds__(128) attention_kv4_join_kernel(const AttArgs a
     }
 }
 
-// Thread blocks along the sequence: enough for two to an SM, each with at least two tiles per warp.
-int pick_splits(int64_t blocks, int max_len) {
+// Thread blocks along the sequence: as many as are resident at once (a second wave would run next to nothing: 4 x 8
+// heads x 32768 tokens in 320 blocks on 296 places took 133 us, in 256 blocks xx), each with at least two
+// tiles per warp.
+int pick_splits(int64_t blocks, int max_len, int ng, int nt) {
     const int sms = sm_count() > 0 ? sm_count() : 148;
-    int64_t s = (2 * sms + blocks - 1) / blocks;
+    int64_t s = blocks_per_sm(ng, nt) * sms / blocks;
     const int64_t most = (max_len + 2 * WARPS * TILE - 1) / (2 * WARPS * TILE);
     s = s < most ? s : most;
     return static_cast<int>(s < 1 ? 1 : (s > MAX_SPLITS ? MAX_SPLITS : s));
 }
 
 struct AttPlan {
-    int rt, tiles, splits;
+    int nt, tiles, splits;
     size_t part, ml;
 };
 AttPlan plan_att(const Kv4View& v, int batch, int seq, int nhead, int max_len) {
     AttPlan p;
     const int64_t rows = static_cast<int64_t>(seq) * (nhead / v.nkv);
-    p.rt = rows > 8 ? 2 : 1;
-    p.tiles = static_cast<int>((rows + 8 * p.rt - 1) / (8 * p.rt));
-    p.splits = pick_splits(static_cast<int64_t>(p.tiles) * v.nkv * batch, max_len);
+    p.nt = rows > 8 ? 2 : 1;
+    p.tiles = static_cast<int>((rows + 8 * p.nt - 1) / (8 * p.nt));
+    p.splits = pick_splits(static_cast<int64_t>(p.tiles) * v.nkv * batch, max_len, v.ng, p.nt);
     const size_t all = static_cast<size_t>(batch) * seq * nhead;
     p.part = p.splits > 1 ? p.splits * all * 32 * v.ng * sizeof(float) : 0;
     p.ml = p.splits > 1 ? p.splits * all * 2 * sizeof(float) : 0;
     return p;
 }
 
-template <int NG, int RT>
+template <int NG, int NT>
 int launch_att(const AttArgs& a, cudaStream_t stream) {
-    auto kern = attention_kv4_kernel<NG, RT>;
+    auto kern = attention_kv4_kernel<NG, NT>;
     static std::atomic<bool> attr_set[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
@@ -648,7 +702,7 @@ int et_attention_kv4_fwd(const et_kv4_t* cache, const et_half* Q, et_half* Z, co
     a.err_word = et::device_error_word();
     if (!a.err_word) return ET_ERR_NO_DEVICE;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    switch (a.c.ng * 2 + p.rt) {
+    switch (a.c.ng * 2 + p.nt) {
         case 3: st = et::launch_att<1, 1>(a, s); break;
         case 4: st = et::launch_att<1, 2>(a, s); break;
         case 5: st = et::launch_att<2, 1>(a, s); break;
