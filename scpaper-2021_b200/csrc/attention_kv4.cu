@@ -13,8 +13,8 @@
 // the magnitude of V.
 //
 // A thread block owns up to 16 query rows that share a key/value head (the heads of a group times the query
-// tokens) and a chunk of the sequence; its four warps take 32-token tiles in turn, each with a ring of bulk copies
-// of its own (page contents land in shared memory as they are; no thread waits for another warp in the
+// tokens) and a chunk of the sequence; its four warps take 32-token tiles in turn, each with a ring of asynchronous
+// copies of its own (page contents land in shared memory as they are; no thread waits for another warp in the
 // loop).  With few rows the sequence is split over blocks whose partial results a second kernel joins.
 //
 // Layout.  Both products have the cache as their 16-row operand and eight query rows as their 8-column one: a few
@@ -55,6 +55,15 @@ struct AttArgs {
     int* err_word;
 };
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {  // 16, or 0: zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // NG 32-bit words at p (shared memory, 4 NG-byte aligned)
 template <int NG>
 __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[NG]) {
@@ -93,20 +102,15 @@ struct Smem {
     static constexpr int CODES = TILE * 16 * NG, PARAMS = TILE * 4 * NG;
     static constexpr int STAGE = 2 * (CODES + PARAMS);  // K codes, V codes, K params, V params
     static constexpr int RING = STAGES * STAGE;
-    static constexpr int WIDE = TILE * NG * 16;  // (s, s, m, m) of K, then of V, as fp32
-    static constexpr int WARP = RING + WIDE;
-    static constexpr int BARS = WARPS * WARP;
-    static constexpr int TOTAL = BARS + WARPS * STAGES * 8 + 16;
+    // (s, s, m, m) of K, then of V, as fp32: a token's groups, and a pad that lets eight lanes read eight tokens
+    // without a bank conflict
+    static constexpr int WIDE_LD = NG % 2 ? NG : NG + 1;
+    static constexpr int WARP = RING + TILE * WIDE_LD * 16;
+    static constexpr int TOTAL = WARPS * WARP;
 };
 
 // Thread blocks that share an SM, by registers (and, at two stages of the widest rows, shared memory).
 constexpr int blocks_per_sm(int ng, int nt) { return nt == 1 ? (ng <= 2 ? 5 : 4) : (ng <= 2 ? 4 : 3); }
-
-// Place of (s, s, m, m) of group g and token t: eight lanes that read eight tokens meet no bank conflict.
-template <int NG>
-__device__ __forceinline__ int wide_at(int t, int g) {
-    return NG == 4 ? t * 4 + (g ^ ((t >> 1) & 3)) : NG == 2 ? t * 2 + (g ^ ((t >> 2) & 1)) : t * NG + g;
-}
 
 // Transposes an 8 x 8 matrix of fp16: lane 4 i + j holds row i, columns 2 j and 2 j + 1, before and after.
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
@@ -126,15 +130,6 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
     const int tau = (i >> 1) + 4 * (i & 1);
     uint8_t* ring = smem + warp * S::WARP;
     float4* wide = reinterpret_cast<float4*>(ring + S::RING);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BARS) + warp * STAGES;
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::BARS + WARPS * STAGES * 8);
-    if (lane == 0) {
-        for (int k = 0; k < STAGES; ++k) mbar_init(&bars[k], 1);
-        *abort_flag = 0;
-        fence_barrier_init();
-    }
-    __syncthreads();
-
     pdl_wait();
     pdl_launch_dependents();
 
@@ -182,62 +177,89 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
         return id;
     };
     int pages = page_of(0), pages_next = page_of(16);
-    // Copies of tile n of this warp (called with n = 0, 1, 2, ... in order): lanes 0 .. 7 fetch half tile
-    // `lane & 1` of one of the four arrays each.
-    const int kind = (lane >> 1) & 3;  // K codes, V codes, K params, V params
-    const uint8_t* src = kind < 2 ? a.c.codes[kind] : reinterpret_cast<const uint8_t*>(a.c.params[kind & 1]);
-    const int row_bytes = kind < 2 ? 16 * NG : 4 * NG;
-    const int dst = (kind < 2 ? kind * S::CODES : 2 * S::CODES + (kind & 1) * S::PARAMS) + (lane & 1) * 16 * row_bytes;
-    uint32_t there = 0;  // two bits per issued tile, the newest lowest: which halves were fetched
+    // Copies tile n of this warp (called with n = 0, 1, 2, ... in order), zeros where nothing is to be read: 32 NG
+    // pieces of 16 bytes of either codes, 8 NG of either parameters, the first half of each from the first page.
+    const uint32_t ring32 = smem_u32(ring) + lane * 16;
     auto issue = [&](int n) {
-        there <<= 2;
-        if (n >= mine) return;
-        if (n != 0 && (n & 15) == 0) {
-            pages = pages_next;
-            pages_next = page_of(n + 16);
+        if (n < mine) {
+            if (n != 0 && (n & 15) == 0) {
+                pages = pages_next;
+                pages_next = page_of(n + 16);
+            }
+            const uint32_t st = ring32 + (n % STAGES) * S::STAGE;
+            const int pos = first + (n * WARPS + warp) * TILE;
+            const int id0 = __shfl_sync(0xffffffffu, pages, (n & 15) * 2);
+            const int id1 = __shfl_sync(0xffffffffu, pages, (n & 15) * 2 + 1);
+            const int have0 = id0 < 0 ? 0 : 16, have1 = id1 < 0 ? 0 : 16;
+            const int64_t at0 = kv4_row(a.c, max(id0, 0), pos, kvh), at1 = kv4_row(a.c, max(id1, 0), pos + 16, kvh);
+#pragma unroll
+            for (int of = 0; of < 2; ++of) {
+                const uint8_t* c0 = a.c.codes[of] + at0 * (16 * NG) + lane * 16;
+                const uint8_t* c1 = a.c.codes[of] + at1 * (16 * NG) + lane * 16 - 256 * NG;
+#pragma unroll
+                for (int u = 0; u < NG; ++u) {
+                    const bool hi = u * 32 + lane >= 16 * NG;  // (for even NG the same for all lanes)
+                    cp_async16(st + of * S::CODES + u * 512, (hi ? c1 : c0) + u * 512, hi ? have1 : have0);
+                }
+                if (lane < 8 * NG) {
+                    const uint8_t* base = reinterpret_cast<const uint8_t*>(a.c.params[of]) + lane * 16;
+                    const bool hi = lane >= 4 * NG;
+                    cp_async16(st + 2 * S::CODES + of * S::PARAMS, base + (hi ? at1 * (4 * NG) - 64 * NG : at0 * (4 * NG)),
+                               hi ? have1 : have0);
+                }
+            }
         }
-        const int id = __shfl_sync(0xffffffffu, pages, (n & 15) * 2 + (lane & 1));
-        const uint32_t have = __ballot_sync(0xffffffffu, id >= 0) & 3u;
-        there |= have;
-        uint64_t* bar = &bars[n % STAGES];
-        if (lane == 0) mbar_arrive_expect_tx(bar, __popc(have) * (S::STAGE / 2));
-        __syncwarp();
-        if (lane < 8 && id >= 0) {
-            const int64_t row = kv4_row(a.c, id, first + (n * WARPS + warp) * TILE + (lane & 1) * 16, kvh);
-            bulk_load(ring + (n % STAGES) * S::STAGE + dst, src + row * row_bytes, 16 * row_bytes, bar);
-        }
+        cp_async_commit();  // (an empty group past the last tile, so that the count stays)
     };
 #pragma unroll
     for (int n = 0; n < STAGES - 1; ++n) issue(n);
 
-    // ---- the rows' queries
+    // ---- the rows' queries, scaled by a power of two of their own to at most 2^11: lossless, and room for the
+    // factor 16 that makes up for the nibbles which K's codes are multiplied at (4 bits up, every second pair)
     int limit[NT][2];        // tokens that rows 8 t + 2 j, 8 t + 2 j + 1 see
-    uint32_t qf[NG][NT][4];  // row 8 t + i: features 32 g + 8 j .. + 8
-    uint64_t qs[NG][NT];     // rows 8 t + 2 j, + 1: sums over the group times 2^-24 (the codes carry that factor)
+    uint32_t qf[NG][NT][4];  // row 8 t + i: features 32 g + 8 j .. + 8, in pairs: times 16, 1, 16, 1
+    uint64_t qs[NG][NT];     // rows 8 t + 2 j, + 1: sums over the group, in the units of the first product
+    float unit[NT][2];       // those units times scale and log2(e)
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int r = row0 + 8 * t + i;
         const int qi = r / a.ratio, head = kvh * a.ratio + r % a.ratio;
         const __half* q = a.Q + (static_cast<int64_t>(b) * a.seq + qi) * a.ldq + head * a.c.dh[0] + 8 * j;
+        uint32_t big = 0;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
             uint4 v = make_uint4(0, 0, 0, 0);
             if (qi < nq && 32 * g + 8 * j < a.c.dh[0]) v = __ldcg(reinterpret_cast<const uint4*>(q + 32 * g));
             qf[g][t][0] = v.x, qf[g][t][1] = v.y, qf[g][t][2] = v.z, qf[g][t][3] = v.w;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) big = max(big, max(qf[g][t][k] & 0x7fffu, (qf[g][t][k] >> 16) & 0x7fffu));
+        }
+        big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+        big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        // 2^k, k = 10 - exponent of the largest (0 for rows of zeros and rows that are not finite)
+        const float largest = __half2float(__ushort_as_half(static_cast<unsigned short>(big)));
+        const int k2 = big == 0 || big >= 0x7c00u ? 0 : 137 - static_cast<int>(__float_as_uint(largest) >> 23);
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + k2) << 23);
+        const float down = __uint_as_float(static_cast<uint32_t>(127 + 20 - k2) << 23) * a.scale_log2;  // 2^(20 - k)
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
             float sum = 0.f;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qf[g][t][k]));
-                sum += f.x + f.y;
+                const float x = f.x * up, y = f.y * up;
+                sum += x + y;
+                qf[g][t][k] = k & 1 ? pack_half2(x, y) : pack_half2(16.f * x, 16.f * y);
             }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            sum *= 0x1p-24f;
+            sum *= 0x1p-20f;
             const float s0 = __shfl_sync(0xffffffffu, sum, 8 * j), s1 = __shfl_sync(0xffffffffu, sum, 8 * j + 4);
             qs[g][t] = pack_f32x2(s0, s1);
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+            unit[t][h] = __shfl_sync(0xffffffffu, down, 8 * j + 4 * h);
             const int qr = (row0 + 8 * t + 2 * j + h) / a.ratio;
             // (rows that are not there compute on zero queries and are never stored)
             limit[t][h] = qr >= nq ? (a.mask_kind == ET_MASK_ADDITIVE ? 0 : INT32_MAX)
@@ -247,8 +269,8 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
 
     float acc[NG][2][NT][4];  // [group][u]: features f = 2 u (elements 0, 1) and, times 16, 2 u + 1 (2, 3)
     uint64_t pm[NG][NT];      // sums of p (m + 8 s), two rows
-    float l[NT][2], top[NT][2];
-    float e = -14.f;  // exponent: every s so far is < 2^e
+    float l[NT][2], top[NT][2];  // sum of p, and the reference less e: -inf until the row sees a key
+    float e = -14.f;             // exponent: every s so far is < 2^e
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -262,50 +284,45 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
     }
 
     const uint64_t minus_one = pack_f32x2(-1.f, -1.f);
-    bool ok = true;
     for (int n = 0; n < mine; ++n) {
-        if (!mbar_wait_bounded_warp(&bars[n % STAGES], (n / STAGES) & 1, abort_flag)) {
-            // (copies still in flight must land before the block's shared memory is given up)
-            for (int k = n; k < mine && k < n + STAGES - 1; ++k)
-                for (uint32_t it = 0; it < ET_SPIN_LIMIT && !mbar_try_wait(&bars[k % STAGES], (k / STAGES) & 1); ++it) {
-                }
-            if (lane == 0) report_error(a.err_word, abort_flag, DEV_TIMEOUT_KV4);
-            ok = false;
-            break;
-        }
+        cp_async_wait<STAGES - 2>();
         __syncwarp();
         issue(n + STAGES - 1);  // into the slot that the previous tile left
         const uint8_t* st = ring + (n % STAGES) * S::STAGE;
         const int tok0 = first + (n * WARPS + warp) * TILE;
-        // token `lane` counts: others (past the end, or of a page that is not there) are taken as zeros
-        const bool in = tok0 + lane < end && ((there >> (2 * (STAGES - 1) + (lane >> 4))) & 1u);
 
         // ---- K's (s, m) to fp32; V's largest s, and whether all of V's are finite
-        uint32_t vp[NG];
-        bool odd = false;
-        uint32_t s_top = 0;
+        uint32_t vp[NG], odd_bits = 0, s_top = 0;
         lds_words<NG>(st + 2 * S::CODES + S::PARAMS + lane * 4 * NG, vp);
         {
             uint32_t kp[NG];
             lds_words<NG>(st + 2 * S::CODES + lane * 4 * NG, kp);
+            if (tok0 + lane >= end) {  // not of this sequence, or this block's: counts as zeros
+#pragma unroll
+                for (int g = 0; g < NG; ++g) kp[g] = vp[g] = 0u;
+            }
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                if (!in) kp[g] = vp[g] = 0u;
                 const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&kp[g]));
-                wide[wide_at<NG>(lane, g)] = make_float4(x.x, x.x, x.y, x.y);
-                if (!q4::finite16(vp[g]) || !q4::finite16(vp[g] >> 16)) {
-                    odd = true;
-                    vp[g] = 0u;
-                }
+                wide[lane * S::WIDE_LD + g] = make_float4(x.x, x.x, x.y, x.y);
+                odd_bits |= (vp[g] & 0x7c007c00u) + 0x04000400u;  // (an exponent of all ones carries)
                 s_top = max(s_top, vp[g] & 0x7fffu);
             }
         }
-        odd = __any_sync(0xffffffffu, odd);
+        const bool odd = __any_sync(0xffffffffu, (odd_bits & 0x80008000u) != 0);
+        if (odd) {
+            s_top = 0;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                if (!q4::finite16(vp[g]) || !q4::finite16(vp[g] >> 16)) vp[g] = 0u;
+                s_top = max(s_top, vp[g] & 0x7fffu);
+            }
+        }
         s_top = __reduce_max_sync(0xffffffffu, s_top);
         const float e_new = fmaxf(e, static_cast<float>(static_cast<int>(s_top >> 10) - 14));
         __syncwarp();
 
-        // ---- scores (times 2^-24): [16-token block][token tau, tau + 8][row 2 j, 2 j + 1]
+        // ---- scores, in the row's units: [16-token block][token tau, tau + 8][row 2 j, 2 j + 1]
         float x[2][NT][2][2];
 #pragma unroll
         for (int bk = 0; bk < 2; ++bk) {
@@ -317,14 +334,13 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
             for (int t = 0; t < NT; ++t) sum[t][0] = sum[t][1] = 0;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                uint32_t a0[4], a1[4];
-#pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    a0[p] = (k0[g] >> (4 * p)) & q4::NIBBLES;
-                    a1[p] = (k1[g] >> (4 * p)) & q4::NIBBLES;
-                }
-                const float4 m0 = wide[wide_at<NG>(16 * bk + tau, g)];
-                const float4 m1 = wide[wide_at<NG>(16 * bk + tau + 8, g)];
+                const uint32_t k0h = k0[g] >> 8, k1h = k1[g] >> 8;
+                const uint32_t a0[4] = {k0[g] & q4::NIBBLES, k0[g] & (q4::NIBBLES << 4), k0h & q4::NIBBLES,
+                                        k0h & (q4::NIBBLES << 4)};
+                const uint32_t a1[4] = {k1[g] & q4::NIBBLES, k1[g] & (q4::NIBBLES << 4), k1h & q4::NIBBLES,
+                                        k1h & (q4::NIBBLES << 4)};
+                const float4 m0 = wide[(16 * bk + tau) * S::WIDE_LD + g];
+                const float4 m1 = wide[(16 * bk + tau + 8) * S::WIDE_LD + g];
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     float d[4];
@@ -343,11 +359,11 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
             }
         }
         if (tok0 + TILE > least || a.mask_kind == ET_MASK_ADDITIVE) {
-            const float per_unit = LOG2E / a.scale_log2;
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
+                    const float per_unit = LOG2E / unit[t][h];
                     const __half* mrow =
                         a.mask + static_cast<int64_t>((row0 + 8 * t + 2 * j + h) / a.ratio) * a.ldm;
 #pragma unroll
@@ -363,55 +379,66 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
                 }
         }
 
-        // ---- online softmax
-        bool moved = false;
-        float ref[NT][2], shrink[NT][2];
+        // ---- online softmax.  The reference moves only when a score passes it by 2^6 (or a larger s arrives): the
+        // lanes then need not agree on the tile's maximum, and p s < 2^6 is as good to fp16.
+        float mx[NT][2];
+        bool move = e_new > e;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float mx = fmaxf(fmaxf(x[0][t][0][h], x[0][t][1][h]), fmaxf(x[1][t][0][h], x[1][t][1][h]));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                mx = fmaxf(mx * a.scale_log2, top[t][h]);
-                // a row that has seen nothing yet keeps sums of zero, whatever its reference
-                const float now = mx == -INFINITY ? 0.f : mx;
-                shrink[t][h] = top[t][h] == -INFINITY ? 1.f : exp2f(top[t][h] - now + e - e_new);
-                moved = moved || shrink[t][h] != 1.f;
-                top[t][h] = mx;
-                ref[t][h] = now + e_new;
+                mx[t][h] = fmaxf(fmaxf(x[0][t][0][h], x[0][t][1][h]), fmaxf(x[1][t][0][h], x[1][t][1][h]));
+                mx[t][h] *= unit[t][h];
+                move = move || mx[t][h] > top[t][h] + 6.f;
             }
-        e = e_new;
-        if (__any_sync(0xffffffffu, moved)) {
+        if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                l[t][0] *= shrink[t][0];
-                l[t][1] *= shrink[t][1];
+                float shrink[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float m = fmaxf(mx[t][h], __shfl_xor_sync(0xffffffffu, mx[t][h], 4));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                    m = fmaxf(m, top[t][h]);
+                    // (a row that has seen nothing keeps sums of zero)
+                    shrink[h] = top[t][h] == -INFINITY ? 1.f : exp2f(top[t][h] - m + e - e_new);
+                    top[t][h] = m;
+                    l[t][h] *= shrink[h];
+                }
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    pm[g][t] = mul_f32x2(pm[g][t], pack_f32x2(shrink[t][0], shrink[t][1]));
+                    pm[g][t] = mul_f32x2(pm[g][t], pack_f32x2(shrink[0], shrink[1]));
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) acc[g][k >> 2][t][k & 3] *= shrink[t][k & 1];
+                    for (int k = 0; k < 8; ++k) acc[g][k >> 2][t][k & 3] *= shrink[k & 1];
                 }
             }
+            e = e_new;
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+            for (int h = 0; h < 2; ++h) {
+                const float ref = (top[t][h] == -INFINITY ? 0.f : top[t][h]) + e;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int k = 0; k < 4; ++k) {
                     float& v = x[k >> 1][t][k & 1][h];
-                    v = exp2_approx(fmaf(v, a.scale_log2, -ref[t][h]));
+                    v = exp2_approx(fmaf(v, unit[t][h], -ref));
                     l[t][h] += v;
                 }
+            }
+        uint64_t px[2][NT][2];  // the same, rows in pairs
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                px[k >> 1][t][k & 1] = pack_f32x2(x[k >> 1][t][k & 1][0], x[k >> 1][t][k & 1][1]);
         if (odd) {  // a group of V that is not finite: NaN for the rows that see it, and for no other
             const uint32_t* raw = reinterpret_cast<const uint32_t*>(st + 2 * S::CODES + S::PARAMS);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int tok = 8 * k + tau;
-                if (tok0 + tok >= end || !((there >> (2 * (STAGES - 1) + (tok >> 4))) & 1u)) continue;
+                if (tok0 + tok >= end) continue;
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
                     const uint32_t w = raw[tok * NG + g];
@@ -434,7 +461,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
         for (int g = 0; g < NG; ++g) {
             const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&vp[g]));
             const float m = fmaf(8.f, v.x, v.y);
-            wide[wide_at<NG>(lane, g)] = make_float4(v.x, v.x, m, m);
+            wide[lane * S::WIDE_LD + g] = make_float4(v.x, v.x, m, m);
         }
         __syncwarp();
 
@@ -455,15 +482,15 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
                                f3 = q4::centred16(w0h);
                 const uint32_t g0 = q4::centred(w1), g1 = q4::centred16(w1), g2 = q4::centred(w1h),
                                g3 = q4::centred16(w1h);
-                const float4 m0 = wide[wide_at<NG>(16 * bk + tau, g)];
-                const float4 m1 = wide[wide_at<NG>(16 * bk + tau + 8, g)];
+                const float4 m0 = wide[(16 * bk + tau) * S::WIDE_LD + g];
+                const float4 m1 = wide[(16 * bk + tau + 8) * S::WIDE_LD + g];
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     uint32_t hi[2], lo[2];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const float4& m = h ? m1 : m0;
-                        const uint64_t p = pack_f32x2(x[bk][t][h][0], x[bk][t][h][1]);
+                        const uint64_t p = px[bk][t][h];
                         const uint64_t ps = mul_f32x2(p, pack_f32x2(m.x, m.y));
                         pm[g][t] = fma_f32x2(p, pack_f32x2(m.z, m.w), pm[g][t]);
                         float p0, p1;
@@ -482,12 +509,13 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
             }
         }
     }
-    if (!__syncthreads_and(ok)) return;  // every warp is done with its ring: it becomes the exchange area
+    cp_async_wait<0>();
+    __syncthreads();  // every warp is done with its ring: it becomes the exchange area
 
     // ---- join the warps: [warp][row][D] sums and [warp][row][2] (reference, sum of p)
     float* xs = reinterpret_cast<float*>(smem);
     constexpr int ROWS = 8 * NT;
-    static_assert(WARPS * ROWS * (D + 2) * 4 <= S::BARS, "exchange area");
+    static_assert(WARPS * ROWS * (D + 2) * 4 <= S::TOTAL, "exchange area");
     float* xml = xs + WARPS * ROWS * D;
     auto over_tokens = [](float v) {
         v += __shfl_xor_sync(0xffffffffu, v, 4);
@@ -698,7 +726,7 @@ int et_attention_kv4_fwd(const et_kv4_t* cache, const et_half* Q, et_half* Z, co
     a.rows = seq * a.ratio;
     a.tiles = p.tiles;
     a.splits = p.splits;
-    a.scale_log2 = scale * et::LOG2E * 0x1p24f;
+    a.scale_log2 = scale * et::LOG2E;
     a.err_word = et::device_error_word();
     if (!a.err_word) return ET_ERR_NO_DEVICE;
     cudaStream_t s = static_cast<cudaStream_t>(stream);

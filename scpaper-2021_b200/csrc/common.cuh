@@ -61,7 +61,6 @@ enum : int {
     DEV_TIMEOUT_VO_SOFTMAX = 403,
     DEV_TIMEOUT_FUSE_O = 304,  // the output projection waited for attention outputs that never came
     DEV_TIMEOUT_PEER = 501,  // a rank's flag did not arrive (head-parallel exchange over peer memory)
-    DEV_TIMEOUT_KV4 = 602,  // a copy out of the 4-bit cache did not land
     DEV_BAD_PAGE = 601,  // a cache position past the page table, or a page number outside the cache
 };
 
