@@ -15,7 +15,8 @@
 // A thread block owns up to 16 query rows that share a key/value head (the heads of a group times the query
 // tokens) and a chunk of the sequence; its four warps take 32-token tiles in turn, each with a ring of asynchronous
 // copies of its own (page contents land in shared memory as they are; no thread waits for another warp in the
-// loop).  With few rows the sequence is split over blocks whose partial results a second kernel joins.
+// loop).  With few rows the sequence is split over the blocks of a cluster, which join their partial results
+// through distributed shared memory, or (more than 16) over blocks that leave them to a second kernel.
 //
 // Layout.  Both products have the cache as their 16-row operand and eight query rows as their 8-column one: a few
 // rows then waste little of the tensor core and of the registers (with the rows on the 16 side, half
@@ -36,6 +37,7 @@ constexpr int TILE = 32;      // tokens of a warp's tile
 constexpr int WARPS = 4;
 constexpr int THREADS = 32 * WARPS;
 constexpr int MAX_SPLITS = 64;
+constexpr int MAX_CLUSTER = 16;  // splits that join through distributed shared memory
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct AttArgs {
@@ -117,6 +119,63 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
+}
+
+// Shared memory of this block (a pointer), or of one of the cluster (an address): what join_partials reads.
+__device__ __forceinline__ float2 load2(const float* p) { return *reinterpret_cast<const float2*>(p); }
+__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float2 load2(uint32_t p) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(p));
+    return v;
+}
+__device__ __forceinline__ float4 load4(uint32_t p) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(p));
+    return v;
+}
+
+// Joins n <= N partial results: ml(c) gives the place of part c's (reference, sum of p), x(c) that of eight sums.
+template <int N, typename ML, typename X>
+__device__ __forceinline__ void join_partials(int n, float (&o)[8], float& top, float& sum, ML ml, X x) {
+    float2 m[N];
+    top = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+        m[c] = make_float2(-INFINITY, 0.f);
+        if (c < n) m[c] = load2(ml(c));
+    }
+#pragma unroll
+    for (int c = 0; c < N; ++c) top = fmaxf(top, m[c].x);
+    sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] = 0.f;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+        if (m[c].x == -INFINITY) continue;
+        const float f = exp2f(m[c].x - top);
+        sum = fmaf(m[c].y, f, sum);
+        const auto p = x(c);
+        const float4 u = load4(p), v = load4(p + 16 / (sizeof(p) == 4 ? 1 : 4));
+        o[0] = fmaf(u.x, f, o[0]), o[1] = fmaf(u.y, f, o[1]), o[2] = fmaf(u.z, f, o[2]), o[3] = fmaf(u.w, f, o[3]);
+        o[4] = fmaf(v.x, f, o[4]), o[5] = fmaf(v.y, f, o[5]), o[6] = fmaf(v.z, f, o[6]), o[7] = fmaf(v.w, f, o[7]);
+    }
+}
+__device__ __forceinline__ void store8(float* p, const float (&o)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(o[0], o[1], o[2], o[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(o[4], o[5], o[6], o[7]);
+}
+// Rows that saw no key are zeros.
+__device__ __forceinline__ void store_z(__half* p, const float (&o)[8], float top, float sum) {
+    const float inv = top == -INFINITY ? 0.f : 1.f / sum;
+    uint4 z;
+    z.x = pack_half2(o[0] * inv, o[1] * inv);
+    z.y = pack_half2(o[2] * inv, o[3] * inv);
+    z.z = pack_half2(o[4] * inv, o[5] * inv);
+    z.w = pack_half2(o[6] * inv, o[7] * inv);
+    *reinterpret_cast<uint4*>(p) = z;
 }
 
 // NT: tiles of eight query rows.
@@ -515,7 +574,6 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
     // ---- join the warps: [warp][row][D] sums and [warp][row][2] (reference, sum of p)
     float* xs = reinterpret_cast<float*>(smem);
     constexpr int ROWS = 8 * NT;
-    static_assert(WARPS * ROWS * (D + 2) * 4 <= S::TOTAL, "exchange area");
     float* xml = xs + WARPS * ROWS * D;
     auto over_tokens = [](float v) {
         v += __shfl_xor_sync(0xffffffffu, v, 4);
@@ -548,47 +606,52 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
         }
     }
     __syncthreads();
-    // eight features of a row per thread and step
+    // eight features of a row per thread and step: the warps', then (few splits) the blocks' of a cluster
+    float* mine_x = xml + 2 * WARPS * ROWS;  // this block's sums [row][D] and (reference, sum of p)
+    float* mine_ml = mine_x + ROWS * D;
+    static_assert((WARPS + 1) * ROWS * (D + 2) * 4 <= S::TOTAL, "exchange area");
+    const bool clustered = a.splits > 1 && a.splits <= MAX_CLUSTER;
     for (int u = threadIdx.x; u < ROWS * (D / 8); u += THREADS) {
         const int r = u / (D / 8), d = (u - r * (D / 8)) * 8;
         const int rr = row0 + r, qi = rr / a.ratio, head = kvh * a.ratio + rr % a.ratio;
         if (qi >= nq) continue;
-        float top_all = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) top_all = fmaxf(top_all, xml[2 * (w * ROWS + r)]);
-        float sum = 0.f, o[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = 0.f;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            const float tw = xml[2 * (w * ROWS + r)];
-            if (tw == -INFINITY) continue;
-            const float f = exp2f(tw - top_all);
-            sum = fmaf(xml[2 * (w * ROWS + r) + 1], f, sum);
-            const float* p = xs + (w * ROWS + r) * D + d;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) o[k] = fmaf(p[k], f, o[k]);
-        }
+        float o[8], top_all, sum;
+        join_partials<WARPS>(WARPS, o, top_all, sum, [&](int w) { return xml + 2 * (w * ROWS + r); },
+                             [&](int w) { return xs + (w * ROWS + r) * D + d; });
         const int64_t row = static_cast<int64_t>(b) * a.seq + qi;
-        if (a.splits > 1) {
+        if (clustered) {
+            store8(mine_x + r * D + d, o);
+            if (d == 0) {
+                mine_ml[2 * r] = top_all;
+                mine_ml[2 * r + 1] = sum;
+            }
+        } else if (a.splits > 1) {
             const int64_t at = (static_cast<int64_t>(split) * a.batch * a.seq + row) * a.nhead + head;
+            store8(a.part + at * D + d, o);
             if (d == 0) {
                 a.part_ml[2 * at] = top_all;
                 a.part_ml[2 * at + 1] = sum;
             }
-            float4* p = reinterpret_cast<float4*>(a.part + at * D + d);
-            p[0] = make_float4(o[0], o[1], o[2], o[3]);
-            p[1] = make_float4(o[4], o[5], o[6], o[7]);
         } else if (d < a.c.dh[1]) {
-            const float inv = top_all == -INFINITY ? 0.f : 1.f / sum;
-            uint4 z;
-            z.x = pack_half2(o[0] * inv, o[1] * inv);
-            z.y = pack_half2(o[2] * inv, o[3] * inv);
-            z.z = pack_half2(o[4] * inv, o[5] * inv);
-            z.w = pack_half2(o[6] * inv, o[7] * inv);
-            *reinterpret_cast<uint4*>(a.Z + row * a.ldz + head * a.c.dh[1] + d) = z;
+            store_z(a.Z + row * a.ldz + head * a.c.dh[1] + d, o, top_all, sum);
         }
     }
+    if (!clustered) return;
+    __syncwarp();
+    cluster_sync_all();
+    const uint32_t x32 = smem_u32(mine_x), ml32 = smem_u32(mine_ml);
+    for (int u = threadIdx.x * a.splits + split; u < ROWS * (D / 8); u += a.splits * THREADS) {
+        const int r = u / (D / 8), d = (u - r * (D / 8)) * 8;
+        const int rr = row0 + r, qi = rr / a.ratio, head = kvh * a.ratio + rr % a.ratio;
+        if (qi >= nq || d >= a.c.dh[1]) continue;
+        float o[8], top_all, sum;
+        join_partials<MAX_CLUSTER>(a.splits, o, top_all, sum,
+                                   [&](int c) { return map_to_cta(ml32 + 8 * r, c); },
+                                   [&](int c) { return map_to_cta(x32 + (r * D + d) * 4, c); });
+        store_z(a.Z + (static_cast<int64_t>(b) * a.seq + qi) * a.ldz + head * a.c.dh[1] + d, o, top_all, sum);
+    }
+    __syncwarp();
+    cluster_sync_all();  // (no block leaves while another reads its shared memory)
 }
 
 // Joins the splits' partial results: a warp per (row, head), four features per lane.
@@ -657,8 +720,8 @@ AttPlan plan_att(const Kv4View& v, int batch, int seq, int nhead, int max_len) {
     p.tiles = static_cast<int>((rows + 8 * p.nt - 1) / (8 * p.nt));
     p.splits = pick_splits(static_cast<int64_t>(p.tiles) * v.nkv * batch, max_len, v.ng, p.nt);
     const size_t all = static_cast<size_t>(batch) * seq * nhead;
-    p.part = p.splits > 1 ? p.splits * all * 32 * v.ng * sizeof(float) : 0;
-    p.ml = p.splits > 1 ? p.splits * all * 2 * sizeof(float) : 0;
+    p.part = p.splits > MAX_CLUSTER ? p.splits * all * 32 * v.ng * sizeof(float) : 0;
+    p.ml = p.splits > MAX_CLUSTER ? p.splits * all * 2 * sizeof(float) : 0;
     return p;
 }
 
@@ -669,12 +732,30 @@ int launch_att(const AttArgs& a, cudaStream_t stream) {
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 0 && dev < 64 && !attr_set[dev]) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<NG>::TOTAL) != cudaSuccess)
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<NG>::TOTAL) != cudaSuccess ||
+            cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
             return ET_ERR_CUDA;
         attr_set[dev] = true;
     }
     const dim3 grid(a.splits, a.tiles * a.c.nkv, a.batch);
-    return launch_kernel(kern, grid, dim3(THREADS), Smem<NG>::TOTAL, stream, a) == cudaSuccess ? ET_OK : ET_ERR_CUDA;
+    if (a.splits == 1 || a.splits > MAX_CLUSTER)
+        return launch_kernel(kern, grid, dim3(THREADS), Smem<NG>::TOTAL, stream, a) == cudaSuccess ? ET_OK : ET_ERR_CUDA;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = Smem<NG>::TOTAL;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(a.splits);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    count_launch();
+    return cudaLaunchKernelEx(&cfg, kern, a) == cudaSuccess ? ET_OK : ET_ERR_CUDA;
 }
 
 }  // namespace
@@ -707,7 +788,7 @@ int et_attention_kv4_fwd(const et_kv4_t* cache, const et_half* Q, et_half* Z, co
         return ET_ERR_SHAPE;
     if (!et::aligned16(Q) || !et::aligned16(Z)) return ET_ERR_ALIGNMENT;
     const et::AttPlan p = et::plan_att(a.c, batch, seq, nhead, max_len);
-    if (p.splits > 1) {
+    if (p.splits > et::MAX_CLUSTER) {
         if (!workspace || workspace_bytes < p.part + p.ml) return ET_ERR_WORKSPACE;
         if (!et::aligned16(workspace)) return ET_ERR_ALIGNMENT;
     }
@@ -740,7 +821,7 @@ int et_attention_kv4_fwd(const et_kv4_t* cache, const et_half* Q, et_half* Z, co
         case 9: st = et::launch_att<4, 1>(a, s); break;
         default: st = et::launch_att<4, 2>(a, s); break;
     }
-    if (st != ET_OK || p.splits == 1) return st;
+    if (st != ET_OK || p.splits <= et::MAX_CLUSTER) return st;
     const int64_t all = static_cast<int64_t>(batch) * seq * nhead;
     return et::launch_kernel(et::attention_kv4_join_kernel, dim3(static_cast<unsigned>((all + 3) / 4)), dim3(128), 0, s,
                              a) == cudaSuccess
