@@ -1,9 +1,11 @@
 // Writing fp16 keys and values into the 4-bit cache, and reading them back.
 //
-// Four lanes serve one (token, head) row of K or of V.  Lane j holds features 32 g + 8 j .. + 8 of every group g
-// (16-byte loads and stores on the fp16 side), so a group's range is two shuffles over the four lanes, and in the
-// cache the lane owns the 4 ng consecutive bytes of its features: one store or load per lane (K: word j of
-// each group; V: units 2 j and 2 j + 1 of each group).  Lane g < ng also moves group g's (s, m).
+// Four lanes serve the rows of one (token, head) in K and in V.  Lane j holds features 32 g + 8 j .. + 8 of every group
+// g (16-byte loads and stores on the fp16 side), so a group's range is two shuffles over the four lanes, and in
+// the cache the lane owns the 4 ng consecutive bytes of its features: one store or load per lane (K: word j of
+// each group; V: units 2 j and 2 j + 1 of each group).  Lane g < ng also writes group g's (s, m).  A warp covers
+// eight consecutive tokens of a head: its rows lie together in the cache (ng = 2: 256 bytes of codes, 64 of
+// parameters), and a token's head is a whole line or more of the fp16 side anyway.
 //
 // What bounds it: HBM (2 + 0.625 bytes a value each way).
 #include "kernels.h"
@@ -15,6 +17,20 @@ namespace {
 
 constexpr int KV_THREADS = 256;
 
+// x / d for 0 <= x < 2^31 by a multiplication
+struct FastDiv {
+    uint32_t mul, shift, d;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t d_) : d(d_) {
+        shift = 0;
+        while ((1u << shift) < d && shift < 31) ++shift;
+        mul = static_cast<uint32_t>(((1ull << (31 + shift)) + d - 1) / d);
+    }
+    __host__ __device__ __forceinline__ uint32_t div(uint32_t x) const {
+        return static_cast<uint32_t>((static_cast<uint64_t>(x) * mul) >> (31 + shift));
+    }
+};
+
 struct Kv4Move {
     Kv4View c;
     __half* x[2];  // fp16 K and V
@@ -22,9 +38,8 @@ struct Kv4Move {
     const int* table;
     const int* start;
     const int* len;
-    int table_ld, batch, seq;
-    int rows_per_token;  // 2 nkv
-    int64_t quads;       // rows in all
+    int table_ld, batch, seq, tokens;
+    FastDiv by_heads, by_seq;
     int* err_word;
 };
 
@@ -72,15 +87,29 @@ template <int NG, bool WRITE>
 __global__ void __launch_bounds__(KV_THREADS) kv4_move_kernel(const Kv4Move a) {
     pdl_wait();
     pdl_launch_dependents();
-    const int64_t q = (static_cast<int64_t>(blockIdx.x) * KV_THREADS + threadIdx.x) >> 2;
-    const int j = threadIdx.x & 3;
-    // (the lanes of a row leave together, those past the last row stay for the shuffles)
-    const int token = q < a.quads ? static_cast<int>(q / a.rows_per_token) : 0;
-    const int r = q < a.quads ? static_cast<int>(q - static_cast<int64_t>(token) * a.rows_per_token) : 0;
-    const int b = token / a.seq, i = token - b * a.seq;
-    const int of = r >= a.c.nkv ? 1 : 0, head = r - of * a.c.nkv;
-    const int n = a.len ? __ldcg(a.len + b) : a.seq;
-    bool live = q < a.quads && i < n;
+    // unit: (eight tokens, head, token of the eight), four lanes each
+    const uint32_t unit = blockIdx.x * (KV_THREADS / 32) + (threadIdx.x >> 5);
+    const uint32_t eight = a.by_heads.div(unit);
+    const int head = static_cast<int>(unit - eight * a.by_heads.d);
+    const int lane = threadIdx.x & 31, j = lane & 3;
+    const int64_t token = static_cast<int64_t>(eight) * 8 + (lane >> 2);
+    bool live = token < a.tokens;  // (the lanes that are not stay for the shuffles)
+    const int b = static_cast<int>(a.by_seq.div(live ? static_cast<uint32_t>(token) : 0u));
+    const int i = static_cast<int>(token) - b * a.seq;
+    live = live && i < (a.len ? __ldcg(a.len + b) : a.seq);
+    uint4 v[2][NG];
+    __half* x[2];
+#pragma unroll
+    for (int of = 0; of < 2; ++of) {
+        x[of] = a.x[of] + token * a.ld[of] + head * a.c.dh[of] + 8 * j;
+        if (WRITE)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                v[of][g] = make_uint4(0, 0, 0, 0);
+                if (live && 32 * g + 8 * j < a.c.dh[of])
+                    v[of][g] = __ldcg(reinterpret_cast<const uint4*>(x[of] + 32 * g));
+            }
+    }
     int64_t row = -1;
     if (live) {
         const int64_t pos = static_cast<int64_t>(a.start ? __ldcg(a.start + b) : 0) + i;
@@ -88,56 +117,56 @@ __global__ void __launch_bounds__(KV_THREADS) kv4_move_kernel(const Kv4Move a) {
         row = id < 0 ? -1 : kv4_row(a.c, id, pos, head);
         if (row < 0 && j == 0) atomicCAS(a.err_word, 0, DEV_BAD_PAGE);
     }
-    const int dh = a.c.dh[of];
-    __half* x = a.x[of] + static_cast<int64_t>(token) * a.ld[of] + head * dh + 8 * j;
-    if (WRITE) {
-        live = live && row >= 0;
-        uint4 v[NG];
+    const bool there = live && row >= 0;
+    uint32_t raw[2][NG], sm[2][NG];
+    if (!WRITE) {
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            v[g] = make_uint4(0, 0, 0, 0);
-            if (live && 32 * g + 8 * j < dh) v[g] = __ldcg(reinterpret_cast<const uint4*>(x + 32 * g));
-        }
-        uint32_t w[NG], sm_mine = 0;
+        for (int of = 0; of < 2; ++of) {
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            const bool in = 32 * g + 8 * j < dh;
-            q4::Range range = {INFINITY, -INFINITY, true};
-            if (in) range = q4::range8(v[g]);
-            q4::range_quad(range);
-            const uint32_t sm = 32 * g < dh ? q4::params_of(range) : 0u;
-            w[g] = in ? q4::codes8(v[g], sm) : 0u;
-            if (g == j) sm_mine = sm;
-        }
-        if (live) {
-            uint32_t out[NG];
-            if (of == 0) {
-#pragma unroll
-                for (int g = 0; g < NG; ++g) out[g] = q4::to_pairs(w[g]);
-            } else {
-                units_of_words<NG>(w, out);
-            }
-            store_words<NG>(a.c.codes[of] + row * (16 * NG) + j * (4 * NG), out);
-            if (j < NG) reinterpret_cast<uint32_t*>(a.c.params[of])[row * NG + j] = sm_mine;
-        }
-    } else if (live) {
-        uint32_t w[NG], sm[NG];
-#pragma unroll
-        for (int g = 0; g < NG; ++g) w[g] = sm[g] = 0u;
-        if (row >= 0) {
-            uint32_t raw[NG];
-            load_words<NG>(a.c.codes[of] + row * (16 * NG) + j * (4 * NG), raw);
-            load_words<NG>(reinterpret_cast<const uint8_t*>(a.c.params[of]) + row * (4 * NG), sm);
-            if (of == 0) {
-#pragma unroll
-                for (int g = 0; g < NG; ++g) w[g] = q4::from_pairs(raw[g]);
-            } else {
-                words_of_units<NG>(raw, w);
+            for (int g = 0; g < NG; ++g) raw[of][g] = sm[of][g] = 0u;
+            if (there) {
+                load_words<NG>(a.c.codes[of] + row * (16 * NG) + j * (4 * NG), raw[of]);
+                load_words<NG>(reinterpret_cast<const uint8_t*>(a.c.params[of]) + row * (4 * NG), sm[of]);
             }
         }
+    }
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
-            if (32 * g + 8 * j < dh) *reinterpret_cast<uint4*>(x + 32 * g) = q4::values8(w[g], sm[g]);
+    for (int of = 0; of < 2; ++of) {
+        uint32_t w[NG];
+        if (WRITE) {
+            uint32_t mine = 0;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const bool in = 32 * g + 8 * j < a.c.dh[of];
+                const uint32_t range = q4::range_quad(in ? q4::range8(v[of][g]) : q4::EMPTY_RANGE);
+                const uint32_t p = 32 * g < a.c.dh[of] ? q4::params_of(range) : 0u;
+                w[g] = in ? (of == 0 ? q4::codes8<true>(v[of][g], p) : q4::codes8<false>(v[of][g], p)) : 0u;
+                if (g == j) mine = p;
+            }
+            if (there) {
+                uint32_t out[NG];
+                if (of == 0) {
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) out[g] = w[g];
+                } else {
+                    units_of_words<NG>(w, out);
+                }
+                store_words<NG>(a.c.codes[of] + row * (16 * NG) + j * (4 * NG), out);
+                if (j < NG) reinterpret_cast<uint32_t*>(a.c.params[of])[row * NG + j] = mine;
+            }
+        } else if (live) {
+            if (of == 0) {
+#pragma unroll
+                for (int g = 0; g < NG; ++g) w[g] = raw[of][g];
+            } else {
+                words_of_units<NG>(raw[of], w);
+            }
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+                if (32 * g + 8 * j < a.c.dh[of])
+                    *reinterpret_cast<uint4*>(x[of] + 32 * g) =
+                        of == 0 ? q4::values8<true>(w[g], sm[of][g]) : q4::values8<false>(w[g], sm[of][g]);
+        }
     }
 }
 
@@ -155,10 +184,12 @@ int move(const et_kv4_t* cache, __half* K, __half* V, int ldk, int ldv, const in
     a.ld[0] = ldk, a.ld[1] = ldv;
     a.table = table, a.start = start, a.len = len;
     a.table_ld = table_ld, a.batch = batch, a.seq = seq;
-    a.rows_per_token = 2 * a.c.nkv;
-    a.quads = static_cast<int64_t>(batch) * seq * a.rows_per_token;
-    const int64_t blocks = (a.quads * 4 + KV_THREADS - 1) / KV_THREADS;
-    if (blocks > INT32_MAX) return ET_ERR_SHAPE;
+    a.tokens = batch * seq;
+    a.by_heads = FastDiv(static_cast<uint32_t>(a.c.nkv));
+    a.by_seq = FastDiv(static_cast<uint32_t>(seq));
+    const int64_t units = (static_cast<int64_t>(a.tokens) + 7) / 8 * a.c.nkv;
+    if (units > INT32_MAX - KV_THREADS) return ET_ERR_SHAPE;
+    const int64_t blocks = (units + KV_THREADS / 32 - 1) / (KV_THREADS / 32);
     a.err_word = device_error_word();
     if (!a.err_word) return ET_ERR_NO_DEVICE;
     void (*const kernels[4])(const Kv4Move) = {kv4_move_kernel<1, WRITE>, kv4_move_kernel<2, WRITE>,

@@ -205,23 +205,17 @@ w4_move_kernel(const __half* __restrict__ W, __half* __restrict__ dense, uint32_
     if (PACK) {
         uint4 v = make_uint4(0, 0, 0, 0);
         if (in_row) v = *reinterpret_cast<const uint4*>(W + static_cast<int64_t>(row) * in + k);
-        q4::Range r = {INFINITY, -INFINITY, true};
-        if (in_row) r = q4::range8(v);
-        q4::range_quad(r);
-        for (int d = 4; d < group / 8; d <<= 1) {
-            r.lo = fminf(r.lo, __shfl_xor_sync(0xffffffffu, r.lo, d));
-            r.hi = fmaxf(r.hi, __shfl_xor_sync(0xffffffffu, r.hi, d));
-            r.finite = __shfl_xor_sync(0xffffffffu, r.finite ? 1 : 0, d) != 0 && r.finite;
-        }
+        uint32_t r = q4::range_quad(in_row ? q4::range8(v) : q4::EMPTY_RANGE);
+        for (int d = 4; d < group / 8; d <<= 1) r = q4::range_join(r, __shfl_xor_sync(0xffffffffu, r, d));
         const int first = b * 128 + n * 32 / group * group;  // of the group
         const uint32_t sm = first < in ? q4::params_of(r) : 0u;
         if (live) {
-            *word = in_row ? q4::to_pairs(q4::codes8(v, sm)) : 0u;
+            *word = in_row ? q4::codes8<true>(v, sm) : 0u;
             if (l % (group / 8) == 0) *pair = sm;
         }
     } else if (in_row) {
         *reinterpret_cast<uint4*>(dense + static_cast<int64_t>(row) * in + k) =
-            q4::values8(q4::from_pairs(*word), *pair);
+            q4::values8<true>(*word, *pair);
     }
 }
 

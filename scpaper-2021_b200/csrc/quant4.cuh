@@ -54,103 +54,97 @@ __device__ __forceinline__ void mma0(float (&d)[4], uint32_t a0, uint32_t a1, ui
 
 __device__ __forceinline__ bool finite16(uint32_t h) { return (h & 0x7c00u) != 0x7c00u; }
 
-// Smallest and largest of a group and whether all of it is finite; combined over lanes by the caller.
-struct Range {
-    float lo, hi;
-    bool finite;
-};
+// Smallest value and the largest's negative of a group, as an fp16 pair; NaN where the group holds one.
+constexpr uint32_t EMPTY_RANGE = 0x7c007c00u;  // (inf, inf)
 
-__device__ __forceinline__ Range range8(const uint4& v) {
-    Range r = {INFINITY, -INFINITY, true};
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        r.finite = r.finite && finite16(w[i]) && finite16(w[i] >> 16);
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        r.lo = fminf(r.lo, fminf(f.x, f.y));
-        r.hi = fmaxf(r.hi, fmaxf(f.x, f.y));
-    }
-    return r;
+__device__ __forceinline__ uint32_t range_join(uint32_t a, uint32_t b) {
+    const __half2 r = __hmin2_nan(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
 }
-
-// Combines the ranges of the four lanes of a group (lanes that differ in their two lowest bits).
-__device__ __forceinline__ void range_quad(Range& r) {
-#pragma unroll
-    for (int d = 1; d <= 2; d <<= 1) {
-        r.lo = fminf(r.lo, __shfl_xor_sync(0xffffffffu, r.lo, d));
-        r.hi = fmaxf(r.hi, __shfl_xor_sync(0xffffffffu, r.hi, d));
-        r.finite = __shfl_xor_sync(0xffffffffu, r.finite ? 1 : 0, d) != 0 && r.finite;
-    }
+__device__ __forceinline__ uint32_t range8(const uint4& v) {
+    const uint32_t lo = range_join(range_join(v.x, v.y), range_join(v.z, v.w));
+    const uint32_t hi = range_join(range_join(v.x ^ 0x80008000u, v.y ^ 0x80008000u),
+                                   range_join(v.z ^ 0x80008000u, v.w ^ 0x80008000u));
+    return range_join(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
+}
+// Joins the ranges of the four lanes of a group of 32 (lanes that differ in their two lowest bits).
+__device__ __forceinline__ uint32_t range_quad(uint32_t r) {
+    r = range_join(r, __shfl_xor_sync(0xffffffffu, r, 1));
+    return range_join(r, __shfl_xor_sync(0xffffffffu, r, 2));
 }
 
 // (s, m) of a group as fp16 bits, s in the low half.  Every step is one IEEE operation.
-__device__ __forceinline__ uint32_t params_of(const Range& r) {
-    if (!r.finite) return 0x7fff7fffu;  // NaN, NaN
-    const __half s = __float2half_rn(__fdiv_rn(__fsub_rn(r.hi, r.lo), 15.f));
-    return static_cast<uint32_t>(__half_as_ushort(s)) |
-           (static_cast<uint32_t>(__half_as_ushort(__float2half_rn(r.lo))) << 16);
+__device__ __forceinline__ uint32_t params_of(uint32_t range) {
+    if (!finite16(range) || !finite16(range >> 16)) return 0x7fff7fffu;  // NaN, NaN
+    const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&range));
+    const __half s = __float2half_rn(__fdiv_rn(__fsub_rn(-r.y, r.x), 15.f));
+    return static_cast<uint32_t>(__half_as_ushort(s)) | (range << 16);
 }
 
-// round_half_even((x - m) / s) limited to 0 .. 15, of the exact quotient: the fp32 estimate is off by less
-// than 1e-5, and what lies within 1e-3 of a border between two codes is decided in 64 bits, where x - m and
-// (c + 1/2) s are exact (fp16 inputs: 41 and 16 bits).
-__device__ __forceinline__ uint32_t code_of(float x, float m, float s, float inv) {
-    const float t = (x - m) * inv;
-    const float f = floorf(t);
-    float c = rintf(t);
-    if (fabsf(t - f - 0.5f) < 1e-3f) {
-        const double e = (static_cast<double>(x) - m) - (static_cast<double>(f) + 0.5) * s;
-        c = e > 0.0 || (e == 0.0 && (static_cast<int>(f) & 1)) ? f + 1.f : f;
-    }
-    return static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f));
-}
-
-// Codes of eight fp16 values, value k in bits 4 k .. 4 k + 3 of the result.
+// Codes of eight fp16 values: round_half_even((x - m) / s) limited to 0 .. 15, of the exact quotient.  The fp32
+// estimate (x - m)(1 / s) is off by less than 2e-6, and where it lies within 1e-5 of a border between two codes, as
+// its remainder tells, the group is done again in 64 bits, where x - m and (c + 1/2) s are exact (fp16 inputs: 41
+// and 16 bits).  Value k goes to nibble k, or (PAIRS) to (k >> 1) + 4 (k & 1).
+template <bool PAIRS>
 __device__ __forceinline__ uint32_t codes8(const uint4& v, uint32_t sm) {
-    const float s = __half2float(__ushort_as_half(static_cast<unsigned short>(sm & 0xffffu)));
-    const float m = __half2float(__ushort_as_half(static_cast<unsigned short>(sm >> 16)));
+    const float2 sm32 = __half22float2(*reinterpret_cast<const __half2*>(&sm));
+    const float s = sm32.x, m = sm32.y;
     if (!(s > 0.f)) return 0u;  // a constant group, or one that is not finite
+    constexpr float MAGIC = 12582912.f;  // 1.5 2^23: sums with it are rounded to whole numbers, in their lowest bits
     const float inv = __frcp_rn(s);
+    const uint64_t inv2 = pack_f32x2(inv, inv), m2 = pack_f32x2(-m, -m), s2 = pack_f32x2(-s, -s);
+    const uint64_t magic2 = pack_f32x2(MAGIC, MAGIC), back2 = pack_f32x2(-MAGIC, -MAGIC);
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    uint32_t out = 0;
+    uint32_t c[8];
+    float worst = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        out |= code_of(f.x, m, s, inv) << (8 * i);
-        out |= code_of(f.y, m, s, inv) << (8 * i + 4);
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        const uint64_t d = add_f32x2(pack_f32x2(x.x, x.y), m2);
+        float u0, u1, e0, e1;
+        unpack_f32x2(fma_f32x2(d, inv2, magic2), u0, u1);
+        u0 = fminf(u0, MAGIC + 15.f);
+        u1 = fminf(u1, MAGIC + 15.f);
+        unpack_f32x2(fma_f32x2(add_f32x2(pack_f32x2(u0, u1), back2), s2, d), e0, e1);
+        worst = fmaxf(worst, fmaxf(fabsf(e0), fabsf(e1)));
+        c[2 * i] = __float_as_uint(u0);
+        c[2 * i + 1] = __float_as_uint(u1);
     }
+    if (worst > 0.49999f * s) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const double d = static_cast<double>(__half2float(__ushort_as_half(
+                                 static_cast<unsigned short>(w[k >> 1] >> (16 * (k & 1)))))) - m;
+            const double f = floor(d * inv);  // (within 1e-5 of the quotient: exact next to a border)
+            const double e = d - (f + 0.5) * s;
+            const int n = static_cast<int>(f);
+            c[k] = static_cast<uint32_t>(max(0, min(15, n + (e > 0.0 || (e == 0.0 && (n & 1))))));
+        }
+    }
+    // nibbles from the highest down; a float's other bits are shifted out or masked away
+    uint32_t out = 0;
+#pragma unroll
+    for (int n = 7; n >= 0; --n) out = out * 16 + (c[PAIRS ? 2 * (n & 3) + (n >> 2) : n] & 15u);
     return out;
 }
 
-// Natural nibble order (value k in nibble k) -> pair order (value k in nibble (k >> 1) + 4 (k & 1)), and back.
-__device__ __forceinline__ uint32_t to_pairs(uint32_t w) {
-    uint32_t r = 0;
-#pragma unroll
-    for (int p = 0; p < 4; ++p) r |= ((w >> (8 * p)) & 0xfu) << (4 * p) | ((w >> (8 * p + 4)) & 0xfu) << (4 * p + 16);
-    return r;
-}
-__device__ __forceinline__ uint32_t from_pairs(uint32_t w) {
-    uint32_t r = 0;
-#pragma unroll
-    for (int p = 0; p < 4; ++p) r |= ((w >> (4 * p)) & 0xfu) << (8 * p) | ((w >> (4 * p + 16)) & 0xfu) << (8 * p + 4);
-    return r;
+// fp16(c s + m), rounded once and limited to 65504 (s is rounded, so 15 s + m may pass it); NaN stays.
+__device__ __forceinline__ uint32_t value2(uint32_t code_pair, __half2 s, __half2 m) {
+    const uint32_t c = and_or(code_pair, NIBBLES, 0x64006400u);
+    const __half2 base = __floats2half2_rn(1024.f, 1024.f), most = __floats2half2_rn(65504.f, 65504.f);
+    const __half2 v = __hmin2_nan(__hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), base), s, m), most);
+    return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// fp16(c s + m), limited to +-65504 (s is rounded, so 15 s + m may pass the type's largest value); NaN stays.
-__device__ __forceinline__ float value_of(uint32_t c, float s, float m) {
-    const float v = fmaf(static_cast<float>(c), s, m);
-    return v > 65504.f ? 65504.f : v;
-}
-
-// Eight values of a word in natural nibble order.
+// Eight values of a word whose value k is in nibble k, or (PAIRS) in (k >> 1) + 4 (k & 1).
+template <bool PAIRS>
 __device__ __forceinline__ uint4 values8(uint32_t w, uint32_t sm) {
-    const float s = __half2float(__ushort_as_half(static_cast<unsigned short>(sm & 0xffffu)));
-    const float m = __half2float(__ushort_as_half(static_cast<unsigned short>(sm >> 16)));
-    uint32_t o[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        o[i] = pack_half2(value_of((w >> (8 * i)) & 0xfu, s, m), value_of((w >> (8 * i + 4)) & 0xfu, s, m));
-    return make_uint4(o[0], o[1], o[2], o[3]);
+    const __half2 pair = *reinterpret_cast<const __half2*>(&sm);
+    const __half2 s = __low2half2(pair), m = __high2half2(pair);
+    const uint32_t a = value2(w, s, m), b = value2(w >> 4, s, m), c = value2(w >> 8, s, m), d = value2(w >> 12, s, m);
+    if (PAIRS) return make_uint4(a, b, c, d);
+    return make_uint4(__byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410), __byte_perm(a, b, 0x7632),
+                      __byte_perm(c, d, 0x7632));
 }
 
 }  // namespace q4
