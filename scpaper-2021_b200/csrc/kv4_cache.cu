@@ -130,6 +130,36 @@ __global__ void __launch_bounds__(KV_THREADS) kv4_move_kernel(const Kv4Move a) {
             }
         }
     }
+    float inv[2][NG];
+    if (WRITE) {
+        // The lanes of a row share the ranges out: after two exchanges lane j holds the whole range of every fourth
+        // (tensor, group), makes its (s, m) and 1 / s, and the others fetch them.
+        constexpr int N = (2 * NG + 3) / 4 * 4;
+        uint32_t r[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int of = k / NG, g = k % NG;
+            r[k] = k < 2 * NG && 32 * g + 8 * j < a.c.dh[of & 1] ? q4::range8(v[of & 1][g]) : q4::EMPTY_RANGE;
+        }
+#pragma unroll
+        for (int k = 0; k < N; k += 4) {
+            const bool one = (j & 1) != 0, two = (j & 2) != 0;
+            const uint32_t lo = q4::range_join(one ? r[k + 1] : r[k],
+                                               __shfl_xor_sync(0xffffffffu, one ? r[k] : r[k + 1], 1));
+            const uint32_t hi = q4::range_join(one ? r[k + 3] : r[k + 2],
+                                               __shfl_xor_sync(0xffffffffu, one ? r[k + 2] : r[k + 3], 1));
+            const uint32_t mine = q4::range_join(two ? hi : lo, __shfl_xor_sync(0xffffffffu, two ? lo : hi, 2));
+            const uint32_t p = mine == q4::EMPTY_RANGE ? 0u : q4::params_of(mine);
+            const float i1 = q4::inverse_of(p);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (k + q < 2 * NG) {
+                    const int of = (k + q) / NG, g = (k + q) % NG;
+                    sm[of][g] = __shfl_sync(0xffffffffu, p, q, 4);
+                    inv[of][g] = __shfl_sync(0xffffffffu, i1, q, 4);
+                }
+        }
+    }
 #pragma unroll
     for (int of = 0; of < 2; ++of) {
         uint32_t w[NG];
@@ -137,11 +167,10 @@ __global__ void __launch_bounds__(KV_THREADS) kv4_move_kernel(const Kv4Move a) {
             uint32_t mine = 0;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const bool in = 32 * g + 8 * j < a.c.dh[of];
-                const uint32_t range = q4::range_quad(in ? q4::range8(v[of][g]) : q4::EMPTY_RANGE);
-                const uint32_t p = 32 * g < a.c.dh[of] ? q4::params_of(range) : 0u;
-                w[g] = in ? (of == 0 ? q4::codes8<true>(v[of][g], p) : q4::codes8<false>(v[of][g], p)) : 0u;
-                if (g == j) mine = p;
+                const uint32_t c = of == 0 ? q4::codes8<true>(v[of][g], sm[of][g], inv[of][g])
+                                           : q4::codes8<false>(v[of][g], sm[of][g], inv[of][g]);
+                w[g] = 32 * g + 8 * j < a.c.dh[of] ? c : 0u;
+                if (g == j) mine = sm[of][g];
             }
             if (there) {
                 uint32_t out[NG];

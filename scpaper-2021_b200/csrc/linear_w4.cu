@@ -210,7 +210,7 @@ w4_move_kernel(const __half* __restrict__ W, __half* __restrict__ dense, uint32_
         const int first = b * 128 + n * 32 / group * group;  // of the group
         const uint32_t sm = first < in ? q4::params_of(r) : 0u;
         if (live) {
-            *word = in_row ? q4::codes8<true>(v, sm) : 0u;
+            *word = in_row ? q4::codes8<true>(v, sm, q4::inverse_of(sm)) : 0u;
             if (l % (group / 8) == 0) *pair = sm;
         }
     } else if (in_row) {

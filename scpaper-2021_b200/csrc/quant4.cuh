@@ -81,17 +81,23 @@ __device__ __forceinline__ uint32_t params_of(uint32_t range) {
     return static_cast<uint32_t>(__half_as_ushort(s)) | (range << 16);
 }
 
+// What codes8 needs of a group: computed once, by one of the lanes that share the group.
+__device__ __forceinline__ float inverse_of(uint32_t sm) {
+    const float s = __half2float(__ushort_as_half(static_cast<unsigned short>(sm & 0xffffu)));
+    return s > 0.f ? __frcp_rn(s) : 0.f;
+}
+
 // Codes of eight fp16 values: round_half_even((x - m) / s) limited to 0 .. 15, of the exact quotient.  The fp32
-// estimate (x - m)(1 / s) is off by less than 2e-6, and where it lies within 1e-5 of a border between two codes, as
-// its remainder tells, the group is done again in 64 bits, where x - m and (c + 1/2) s are exact (fp16 inputs: 41
-// and 16 bits).  Value k goes to nibble k, or (PAIRS) to (k >> 1) + 4 (k & 1).
+// estimate (x - m)(1 / s) is off by less than 2e-6; where it lies within 1e-5 of a border between two codes, as its
+// remainder tells, the eight are done again in 64 bits, where x - m and (c + 1/2) s are exact (fp16 inputs: 41
+// and 16 bits).  So are groups with s below 2^-19, whose rounding (to a grid of 2^-24) can leave quotients above
+// 15.5; elsewhere the largest is 15.23.  Value k goes to nibble k, or (PAIRS) to (k >> 1) + 4 (k & 1).
 template <bool PAIRS>
-__device__ __forceinline__ uint32_t codes8(const uint4& v, uint32_t sm) {
+__device__ __forceinline__ uint32_t codes8(const uint4& v, uint32_t sm, float inv) {
     const float2 sm32 = __half22float2(*reinterpret_cast<const __half2*>(&sm));
     const float s = sm32.x, m = sm32.y;
-    if (!(s > 0.f)) return 0u;  // a constant group, or one that is not finite
     constexpr float MAGIC = 12582912.f;  // 1.5 2^23: sums with it are rounded to whole numbers, in their lowest bits
-    const float inv = __frcp_rn(s);
+    constexpr uint32_t MAGIC_BITS = 0x4b400000u;
     const uint64_t inv2 = pack_f32x2(inv, inv), m2 = pack_f32x2(-m, -m), s2 = pack_f32x2(-s, -s);
     const uint64_t magic2 = pack_f32x2(MAGIC, MAGIC), back2 = pack_f32x2(-MAGIC, -MAGIC);
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -101,31 +107,31 @@ __device__ __forceinline__ uint32_t codes8(const uint4& v, uint32_t sm) {
     for (int i = 0; i < 4; ++i) {
         const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
         const uint64_t d = add_f32x2(pack_f32x2(x.x, x.y), m2);
+        const uint64_t u = fma_f32x2(d, inv2, magic2);
         float u0, u1, e0, e1;
-        unpack_f32x2(fma_f32x2(d, inv2, magic2), u0, u1);
-        u0 = fminf(u0, MAGIC + 15.f);
-        u1 = fminf(u1, MAGIC + 15.f);
-        unpack_f32x2(fma_f32x2(add_f32x2(pack_f32x2(u0, u1), back2), s2, d), e0, e1);
+        unpack_f32x2(u, u0, u1);
+        unpack_f32x2(fma_f32x2(add_f32x2(u, back2), s2, d), e0, e1);
         worst = fmaxf(worst, fmaxf(fabsf(e0), fabsf(e1)));
         c[2 * i] = __float_as_uint(u0);
         c[2 * i + 1] = __float_as_uint(u1);
     }
-    if (worst > 0.49999f * s) {
+    if (worst > (s < 0x1p-19f ? -1.f : 0.49999f * s) && s > 0.f) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const double d = static_cast<double>(__half2float(__ushort_as_half(
                                  static_cast<unsigned short>(w[k >> 1] >> (16 * (k & 1)))))) - m;
-            const double f = floor(d * inv);  // (within 1e-5 of the quotient: exact next to a border)
+            const double f = floor(d * inv);  // (next to a border that is the number below it)
             const double e = d - (f + 0.5) * s;
             const int n = static_cast<int>(f);
-            c[k] = static_cast<uint32_t>(max(0, min(15, n + (e > 0.0 || (e == 0.0 && (n & 1))))));
+            c[k] = MAGIC_BITS + max(0, min(15, n + (e > 0.0 || (e == 0.0 && (n & 1)))));
         }
     }
-    // nibbles from the highest down; a float's other bits are shifted out or masked away
+    // nibbles from the highest down; what the floats' other bits add up to is a constant
     uint32_t out = 0;
 #pragma unroll
-    for (int n = 7; n >= 0; --n) out = out * 16 + (c[PAIRS ? 2 * (n & 3) + (n >> 2) : n] & 15u);
-    return out;
+    for (int n = 7; n >= 0; --n) out = out * 16 + c[PAIRS ? 2 * (n & 3) + (n >> 2) : n];
+    out -= MAGIC_BITS * 0x11111111u;
+    return s > 0.f ? out : 0u;  // a constant group, or one that is not finite: 0
 }
 
 // fp16(c s + m), rounded once and limited to 65504 (s is rounded, so 15 s + m may pass it); NaN stays.
