@@ -181,36 +181,52 @@ struct PackedExpander {
 // The same for 4-bit codes: every element of the 16 rows is written.  A code becomes fp16 exactly (1024 + c,
 // less 1024), and c s + m is rounded to fp16 once: the tensor core cannot scale its sums per group, so the
 // operand has to carry the scale.  Lane 4 i + j expands words 2 q and 2 q + 1 (q: which half of the 128-feature
-// block) of rows i and i + 8, fetched one block ahead.
+// block) of rows i and i + 8, fetched QUANT_AHEAD items ahead (with one, 33 tokens x 8192 -> 8192 took 48 us: a trip to
+// memory per item).
+constexpr int QUANT_AHEAD = 4;
 struct QuantExpander {
-    const uint2* codes;
+    struct Item {
+        uint2 v[2];
+        uint32_t sm[2][2];  // [row half][word]
+    } q[QUANT_AHEAD];
+    const uint2* codes;      // of the next item to fetch
     const uint32_t* params;
-    int nb, nkb, gb, lane;
-    uint2 v[2];
-    uint32_t sm[2][2];  // [row half][word]
+    int next, nkb, gb, lane, step;
 
-    __device__ __forceinline__ void fetch(int kb) {
-        if (kb >= nkb) return;
-        const int b = kb >> 1, q = kb & 1;
+    __device__ __forceinline__ void fetch(Item& x) {
+        if (next < nkb) {
+            const int h2 = next & 1;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            v[h] = __ldg(codes + ((static_cast<size_t>(b) * 2 + h) * 32 + lane) * 2 + q);
-            const uint32_t* p = params + (static_cast<size_t>(b) * 16 + 8 * h + (lane >> 2)) * gb;
-            sm[h][0] = __ldg(p + ((2 * q) * gb >> 2));
-            sm[h][1] = __ldg(p + ((2 * q + 1) * gb >> 2));
+            for (int h = 0; h < 2; ++h) {
+                x.v[h] = __ldg(codes + h * 64 + h2);
+                x.sm[h][0] = __ldg(params + h * 8 * gb + ((2 * h2 * gb) >> 2));
+                x.sm[h][1] = __ldg(params + h * 8 * gb + (((2 * h2 + 1) * gb) >> 2));
+            }
+            // the block of the next item: (step + the item's own half) / 2 further on
+            const int blocks = (h2 + step) >> 1;
+            codes += blocks * 128;
+            params += blocks * 16 * gb;
         }
+        next += step;
     }
     __device__ __forceinline__ void init(const ExpandArgs& a, int panel, int lane_) {
         lane = lane_;
-        nb = (a.in + 127) >> 7;
+        const int nb = (a.in + 127) >> 7;
         nkb = (a.in + BK - 1) / BK;
         gb = 128 / a.group;
-        codes = reinterpret_cast<const uint2*>(a.data) + static_cast<size_t>(panel) * nb * 128;
-        params = reinterpret_cast<const uint32_t*>(a.idx0) + static_cast<size_t>(panel) * nb * 16 * gb;
+        codes = reinterpret_cast<const uint2*>(a.data) + static_cast<size_t>(panel) * nb * 128 + lane * 2;
+        params = reinterpret_cast<const uint32_t*>(a.idx0) + static_cast<size_t>(panel) * nb * 16 * gb + (lane >> 2) * gb;
     }
-    __device__ __forceinline__ void start(int kb, int) { fetch(kb); }
-    __device__ __forceinline__ void write(uint8_t* tile, int kb, int step) {
-        if (kb >= nkb) return;
+    __device__ __forceinline__ void start(int kb, int step_) {
+        step = step_;
+        next = kb;
+        codes += (kb >> 1) * 128;
+        params += (kb >> 1) * 16 * gb;
+#pragma unroll
+        for (int u = 0; u < QUANT_AHEAD; ++u) fetch(q[u]);
+    }
+    // expands one item of the ring into `tile` and fills its place again
+    __device__ __forceinline__ void write(uint8_t* tile, Item& x) {
         const __half2 base = __floats2half2_rn(1024.f, 1024.f);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -218,13 +234,13 @@ struct QuantExpander {
             uint8_t* line = tile + row * 128;
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-                const uint32_t w = n ? v[h].y : v[h].x;
-                const __half2 pair = *reinterpret_cast<const __half2*>(&sm[h][n]);
+                const uint32_t w = n ? x.v[h].y : x.v[h].x;
+                const __half2 pair = *reinterpret_cast<const __half2*>(&x.sm[h][n]);
                 const __half2 s = __low2half2(pair), m = __high2half2(pair);
                 uint32_t o[4];
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
-                    const uint32_t c = ((w >> (4 * p)) & q4::NIBBLES) | 0x64006400u;
+                    const uint32_t c = q4::and_or(w >> (4 * p), q4::NIBBLES, 0x64006400u);
                     const __half2 y = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), base), s, m);
                     o[p] = *reinterpret_cast<const uint32_t*>(&y);
                 }
@@ -232,7 +248,7 @@ struct QuantExpander {
                     make_uint4(o[0], o[1], o[2], o[3]);
             }
         }
-        fetch(kb + step);
+        fetch(x);
     }
 };
 
@@ -476,14 +492,38 @@ linear_expand_kernel(const __grid_constant__ CUtensorMap tmX, const ExpandArgs g
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&b_full[buf]);
             }
+        } else if constexpr (FMT == FMT_QUANT) {
+            // As below, by four items a round, whose registers the compiler then knows by name.
+            constexpr int SETS = BN / 16;
+            const int set = w % SETS, sub = w / SETS;
+            const bool live = n0 + set * 16 < g.out;
+            QuantExpander x;
+            if (live) {
+                x.init(g, (n0 >> 4) + set, lane);
+                x.start(sub, g.ckb);
+            }
+            static_assert(X_MAX_B == QUANT_AHEAD, "a round fills every buffer once");
+            uint32_t bph = 0;
+            for (int c0 = 0; c0 < nchunk; c0 += QUANT_AHEAD, bph ^= 1u)
+#pragma unroll
+                for (int u = 0; u < QUANT_AHEAD; ++u) {
+                    if (c0 + u >= nchunk) break;
+                    if (ok) {
+                        ok = mbar_wait_bounded(&b_empty[u], bph ^ 1, abort_flag);
+                        ok = __all_sync(0xffffffffu, ok);
+                    }
+                    uint8_t* tile = sB + u * buf_bytes + sub * (BN * 128) + set * (16 * 128);
+                    if (live && (c0 + u) * g.ckb + sub < nkb) x.write(tile, x.q[u]);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&b_full[u]);
+                }
         } else {
             // Item (16 output rows, K block) of a buffer per warp: BN / 16 row sets x ckb blocks = 8.
             constexpr int SETS = BN / 16;
             const int set = w % SETS, sub = w / SETS;  // sub < ckb
             const bool live = n0 + set * 16 < g.out;
-            typename std::conditional<
-                FMT == FMT_QUANT, QuantExpander,
-                typename std::conditional<FMT == FMT_VEC, VecExpander, PackedExpander>::type>::type x;
+            typename std::conditional<FMT == FMT_VEC, VecExpander, PackedExpander>::type x;
             if (live) {
                 x.init(g, (n0 >> 4) + set, lane);
                 x.start(sub, g.ckb);
@@ -496,12 +536,10 @@ linear_expand_kernel(const __grid_constant__ CUtensorMap tmX, const ExpandArgs g
                     ok = __all_sync(0xffffffffu, ok);
                 }
                 uint8_t* tile = sB + buf * buf_bytes + sub * (BN * 128) + set * (16 * 128);
-                if (FMT != FMT_QUANT) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        reinterpret_cast<uint4*>(tile)[i * 32 + lane] = make_uint4(0u, 0u, 0u, 0u);
-                    __syncwarp();
-                }
+                for (int i = 0; i < 4; ++i)
+                    reinterpret_cast<uint4*>(tile)[i * 32 + lane] = make_uint4(0u, 0u, 0u, 0u);
+                __syncwarp();
                 if (live) x.write(tile, c * g.ckb + sub, g.ckb);
                 fence_proxy_async_smem();
                 __syncwarp();

@@ -4,13 +4,15 @@
 // Mathematics.  Per group of input features,
 //     y[t, o] = sum_g ( s_g(o) (x_t . c_o)_g + m_g(o) (sum of x_t over g) ),
 // so the tensor core multiplies codes (16 output rows x 16 features, exact) by up to eight fp16 tokens, and
-// scale and minimum are applied to its fp32 sums once per group.  The sums of x come from the same instruction, with
-// an operand of ones in place of the codes: they arrive in the lanes that need them.
+// scale and minimum are applied to its fp32 sums once per group.  The sums of x are made when it is staged, by the
+// same instruction with ones for codes.
+// Nibbles 4 bits up are taken where they are, 16 times as large, into sums of their own.
 //
-// A warp walks blocks of 16 rows x 128 features (1 KB, in lane order: two 16-byte loads a lane) a few blocks
-// ahead in registers; the warps of a thread block share 1, 2 or 4 panels of 16 rows and split the features among
-// them, adding up in shared memory.  Activations are staged there too, in chunks when they do not fit.
-// Weights do not depend on earlier kernels: the first blocks are fetched before the wait for them.
+// A warp walks blocks of 16 rows x 128 features (1 KB and their (s, m), in lane order), copied asynchronously up to
+// seven blocks ahead into a ring of its own: most of what an SM reads is then in flight at once.  The warps of a
+// thread block share 1, 2 or 4 panels of 16 rows and split the features among them, adding up in shared
+// memory; a block walks panels until none is left.  Activations are staged in shared memory, in chunks when
+// they do not fit.  Weights do not depend on earlier kernels: the ring is filled before the wait for them.
 #include <atomic>
 
 #include "kernels.h"
@@ -21,170 +23,246 @@ namespace {
 
 constexpr int W4_WARPS = 8;
 constexpr int W4_THREADS = 32 * W4_WARPS;
-// Blocks in flight per warp (32 tokens: fewer, since a chunk of activations holds that many per warp).
-template <int NT>
-constexpr int W4_AHEAD_OF = NT == 4 ? 2 : 4;
-constexpr int W4_X_BYTES = 96 * 1024;     // staged activations at most
-constexpr uint32_t W4_ONES = 0x00010001u; // code 1, twice
+constexpr size_t W4_SMEM = 227 * 1024;
+constexpr uint32_t W4_ONES = 0x00010001u;  // code 1, twice
 
 struct W4Args {
-    const uint4* codes;
+    const uint8_t* codes;
     const __half* params;
     const __half* bias;
     const __half* X;
     __half* Y;
     int T, in, out, act;
     int nb, panels;
-    int wp_log;        // log2 of the panels per thread block
-    int chunk_blocks;  // staged at a time; a multiple of warps along K x blocks in flight
+    int wp_log;        // log2 of the panels that a thread block works on at a time
+    int chunk_blocks;  // of activations staged at a time: a multiple of the warps along K
 };
 
-__device__ __forceinline__ uint4 ld_stream(const uint4* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
-    return v;
+__device__ __forceinline__ void w4_copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-// GB groups per block of 128 features; NT tiles of eight tokens.
-template <int GB, int NT>
+// MP panels of 16 rows to a warp, GB groups per block of 128 features, NT tiles of eight tokens.
+// Shared memory: activations [rows][chunk + 64 bytes], their sums [chunk groups][8 NT], the warps' sums, the rings.
+// (Activation rows lie 64 bytes apart in the banks: eight lanes - two tokens, four pieces - meet no conflict.)
+template <int MP, int GB, int NT>
+struct W4Smem {
+    static constexpr int DEPTH = MP == 2 ? 4 : 8;  // stages of a ring, of 2 or 1 KB of codes
+    static constexpr int STAGE = MP * (1024 + 64 * GB);
+    static constexpr int RINGS = W4_WARPS * DEPTH * STAGE;
+    static constexpr int RED = W4_WARPS * MP * 8 * NT * 16 * 4;
+    static size_t bytes(int rows, int chunk) {
+        return static_cast<size_t>(rows) * (chunk * 256 + 64) + static_cast<size_t>(chunk) * GB * 8 * NT * 4 + RED + RINGS;
+    }
+};
+
+template <int MP, int GB, int NT>
 __global__ void __launch_bounds__(W4_THREADS, NT == 1 ? 2 : 1) linear_w4_kernel(const W4Args a) {
-    constexpr int W4_AHEAD = W4_AHEAD_OF<NT>;
+    using S = W4Smem<MP, GB, NT>;
     extern __shared__ __align__(16) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int i = lane >> 2, j = lane & 3;
     const int wp = 1 << a.wp_log, wk = W4_WARPS >> a.wp_log;
-    const int panel = blockIdx.x * wp + (warp & (wp - 1)), k0 = warp >> a.wp_log;
-    const bool live = panel < a.panels;
-    const int mine = live && a.nb > k0 ? (a.nb - k0 + wk - 1) / wk : 0;  // blocks k0, k0 + wk, ...
+    const int k0 = warp >> a.wp_log, w0 = warp & (wp - 1);
     const int t0 = blockIdx.y * 8 * NT;
     const int nt_live = a.T - t0 < 8 * NT ? a.T - t0 : 8 * NT;
+    const int rows = a.T < 8 * NT ? a.T : 8 * NT;
+    const int ldx = a.chunk_blocks * 256 + 64;
+    float* xsum = reinterpret_cast<float*>(smem + rows * ldx);
+    float* red = xsum + a.chunk_blocks * GB * 8 * NT;
+    uint8_t* ring = reinterpret_cast<uint8_t*>(red) + S::RED + warp * (S::DEPTH * S::STAGE);
 
-    uint4 w[W4_AHEAD][2];
-    uint32_t sm[W4_AHEAD][2][GB];
-    auto fetch = [&](int u, int it) {
-        if (it >= mine) return;
-        const int64_t at = static_cast<int64_t>(panel) * a.nb + k0 + it * wk;
-        w[u][0] = ld_stream(a.codes + at * 64 + lane);
-        w[u][1] = ld_stream(a.codes + at * 64 + 32 + lane);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t* p = reinterpret_cast<const uint32_t*>(a.params) + (at * 16 + 8 * h + i) * GB;
-            if (GB == 4) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-                sm[u][h][0] = v.x, sm[u][h][GB > 1] = v.y, sm[u][h][GB > 2 ? 2 : 0] = v.z, sm[u][h][GB > 3 ? 3 : 0] = v.w;
-            } else if (GB == 2) {
-                const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-                sm[u][h][0] = v.x, sm[u][h][GB > 1] = v.y;
-            } else {
-                sm[u][h][0] = __ldg(p);
+    // ---- the warp's blocks, in order: k0, k0 + wk, ... of units (MP panels) w0, w0 + wp grid, ...
+    const int per_unit = a.nb > k0 ? (a.nb - k0 + wk - 1) / wk : 0;
+    const int units = (a.panels + MP - 1) / MP, groups = (units + wp - 1) / wp;
+    int unit = blockIdx.x * wp + w0, left = per_unit;  // of the next copy: its unit, and the unit's blocks to come
+    uint32_t next_slot = 0;
+    const uint32_t ring32 = smem_u32(ring) + lane * 16;
+    const uint8_t *src, *src_params;
+    int second;  // blocks from the first panel to the second (a last panel without one: that panel again)
+    auto aim = [&]() {
+        const int64_t at = static_cast<int64_t>(unit) * MP * a.nb + k0;
+        second = MP == 2 && unit * MP + 1 < a.panels ? a.nb : 0;
+        src = a.codes + at * 1024 + lane * 16;
+        src_params = reinterpret_cast<const uint8_t*>(a.params) + (at + (lane < 16 ? 0 : second)) * (64 * GB) + (lane & 15) * 16;
+    };
+    aim();
+    auto issue = [&]() {
+        if (unit < units && per_unit > 0) {
+            const uint32_t dst = ring32 + next_slot;
+            w4_copy16(dst, src);
+            w4_copy16(dst + 512, src + 512);
+            if (MP == 2) {
+                w4_copy16(dst + 1024, src + second * 1024ll);
+                w4_copy16(dst + 1536, src + second * 1024ll + 512);
             }
+            if ((lane & 15) < 4 * GB && (MP == 2 || lane < 16))
+                w4_copy16(dst + MP * 1024 - (lane < 16 ? 0 : 256 - 64 * GB), src_params);
+            src += wk * 1024;
+            src_params += wk * (64 * GB);
+            if (--left == 0) {
+                left = per_unit;
+                unit += gridDim.x * wp;
+                aim();
+            }
+            next_slot = next_slot == (S::DEPTH - 1) * S::STAGE ? 0 : next_slot + S::STAGE;
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");  // (empty past the last block, so that the count stays)
     };
 #pragma unroll
-    for (int u = 0; u < W4_AHEAD; ++u) fetch(u, u);
+    for (int u = 0; u < S::DEPTH - 1; ++u) issue();
 
     pdl_wait();
     pdl_launch_dependents();
 
-    float acc[NT][4];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
-
+    int slot = 0;
     const int per_chunk = a.chunk_blocks / wk;  // of a warp
-    // rows 64 bytes apart in the banks: eight lanes of a load (two tokens, four pieces) meet no conflict
-    const int ldx = a.chunk_blocks * 256 + 64;
-    for (int c = 0, b0 = 0; b0 < a.nb; ++c, b0 += a.chunk_blocks) {
-        if (c > 0) __syncthreads();
-        const int blocks = a.nb - b0 < a.chunk_blocks ? a.nb - b0 : a.chunk_blocks;
-        for (int t = warp; t < nt_live; t += W4_WARPS) {
-            const __half* x = a.X + static_cast<int64_t>(t0 + t) * a.in + b0 * 128;
-            const int left = a.in - b0 * 128;
-            for (int p = lane; p < blocks * 16; p += 32) {
-                const bool in = p * 8 < left;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem + t * ldx + p * 16)),
-                             "l"(in ? x + p * 8 : a.X), "r"(in ? 16 : 0)
-                             : "memory");
-            }
-        }
-        asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
-        __syncthreads();
-        const int it0 = c * per_chunk, it1 = it0 + per_chunk < mine ? it0 + per_chunk : mine;
-        for (int it = it0; it < it1; it += W4_AHEAD) {
+    uint8_t* xrow[NT];                          // the lane's tokens; past the last, that one again (never stored)
 #pragma unroll
-            for (int u = 0; u < W4_AHEAD; ++u) {
-                if (it + u < it1) {
-                    const uint8_t* xb = smem + (k0 + (it + u) * wk - b0) * 256 + j * 16;
-                    const uint32_t r0[4] = {w[u][0].x, w[u][0].y, w[u][0].z, w[u][0].w};
-                    const uint32_t r1[4] = {w[u][1].x, w[u][1].y, w[u][1].z, w[u][1].w};
+    for (int t = 0; t < NT; ++t) xrow[t] = smem + (8 * t + i < nt_live ? 8 * t + i : nt_live - 1) * ldx + j * 16;
+    for (int group = blockIdx.x; group < groups; group += gridDim.x) {
+        const bool live = group * wp + w0 < units;
+        float acc[MP][NT][4];
 #pragma unroll
-                    for (int g = 0; g < GB; ++g) {
-                        float d[NT][4], xs[NT][4];
+        for (int k = 0; k < MP * NT * 4; ++k) acc[k / (4 * NT)][k / 4 % NT][k % 4] = 0.f;
+        for (int c = 0, b0 = 0; b0 < a.nb; ++c, b0 += a.chunk_blocks) {
+            // ---- stage activations and their sums over groups (once, if they fit whole)
+            // With one unit at a time a warp reads no features but those of its own blocks, and stages them alone.
+            if (a.nb > a.chunk_blocks || group == static_cast<int>(blockIdx.x)) {
+                if (wp > 1) __syncthreads();
+                else __syncwarp();
+                const int blocks = a.nb - b0 < a.chunk_blocks ? a.nb - b0 : a.chunk_blocks;
+                const int pieces = blocks * 16;
+                const int inside = pieces < (a.in - b0 * 128) / 8 ? pieces : (a.in - b0 * 128) / 8;
+                const __half* x = a.X + static_cast<int64_t>(t0) * a.in + b0 * 128;
+                uint32_t to = smem_u32(smem);
+                // (a warp alone: 16 pieces a block, two blocks at a time)
+                const int p0 = wp > 1 ? threadIdx.x : (warp + (lane >> 4) * W4_WARPS) * 16 + (lane & 15);
+                const int step = wp > 1 ? W4_THREADS : 2 * W4_WARPS * 16;
+                for (int t = 0; t < nt_live; ++t, x += a.in, to += ldx) {
+#pragma unroll 4
+                    for (int p = p0; p < pieces; p += step) {
+                        if (p < inside) w4_copy16(to + p * 16, x + p * 8);
+                        else *reinterpret_cast<uint4*>(smem + t * ldx + p * 16) = make_uint4(0, 0, 0, 0);  // (past the row)
+                    }
+                }
+                asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
+                if (wp > 1) __syncthreads();
+                else __syncwarp();
+                for (int b = warp; b < blocks; b += W4_WARPS) {
 #pragma unroll
-                        for (int t = 0; t < NT; ++t)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) d[t][k] = xs[t][k] = 0.f;
-#pragma unroll
-                        for (int n = g * (4 / GB); n < (g + 1) * (4 / GB); ++n) {
-                            uint32_t A0[4], A1[4];
-#pragma unroll
-                            for (int p = 0; p < 4; ++p) {
-                                A0[p] = (r0[n] >> (4 * p)) & q4::NIBBLES;
-                                A1[p] = (r1[n] >> (4 * p)) & q4::NIBBLES;
-                            }
-#pragma unroll
-                            for (int t = 0; t < NT; ++t) {
-                                uint4 x = make_uint4(0, 0, 0, 0);
-                                if (8 * t + i < nt_live)
-                                    x = *reinterpret_cast<const uint4*>(xb + (8 * t + i) * ldx + n * 64);
-                                q4::mma(d[t], A0[0], A1[0], A0[1], A1[1], x.x, x.y);
-                                q4::mma(d[t], A0[2], A1[2], A0[3], A1[3], x.z, x.w);
-                                q4::mma(xs[t], W4_ONES, W4_ONES, W4_ONES, W4_ONES, x.x, x.y);
-                                q4::mma(xs[t], W4_ONES, W4_ONES, W4_ONES, W4_ONES, x.z, x.w);
-                            }
-                        }
-                        const float2 p0 = __half22float2(*reinterpret_cast<const __half2*>(&sm[u][0][g]));
-                        const float2 p1 = __half22float2(*reinterpret_cast<const __half2*>(&sm[u][1][g]));
+                    for (int g = 0; g < GB; ++g)
 #pragma unroll
                         for (int t = 0; t < NT; ++t) {
-                            acc[t][0] = fmaf(d[t][0], p0.x, fmaf(xs[t][0], p0.y, acc[t][0]));
-                            acc[t][1] = fmaf(d[t][1], p0.x, fmaf(xs[t][1], p0.y, acc[t][1]));
-                            acc[t][2] = fmaf(d[t][2], p1.x, fmaf(xs[t][0], p1.y, acc[t][2]));
-                            acc[t][3] = fmaf(d[t][3], p1.x, fmaf(xs[t][1], p1.y, acc[t][3]));
+                            float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (int n = g * (4 / GB); n < (g + 1) * (4 / GB); ++n) {
+                                uint4* at = reinterpret_cast<uint4*>(xrow[t] + b * 256 + n * 64);
+                                const uint4 x = *at;
+                                q4::mma(d, W4_ONES, W4_ONES, W4_ONES, W4_ONES, x.x, x.y);
+                                q4::mma(d, W4_ONES, W4_ONES, W4_ONES, W4_ONES, x.z, x.w);
+                                // pairs 0 and 2, 1 and 3 together: the second operand's registers below
+                                if (8 * t + i < nt_live) *at = make_uint4(x.x, x.z, x.y, x.w);
+                            }
+                            if (i == 0)
+                                *reinterpret_cast<float2*>(xsum + (b * GB + g) * (8 * NT) + 8 * t + 2 * j) =
+                                    make_float2(d[0], d[1]);
+                        }
+                }
+                if (wp > 1) __syncthreads();
+                else __syncwarp();
+            }
+            const int it0 = c * per_chunk, it1 = it0 + per_chunk < per_unit ? it0 + per_chunk : per_unit;
+            for (int it = it0; live && it < it1; ++it) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(S::DEPTH - 2) : "memory");
+                __syncwarp();
+                issue();  // into the slot that the previous block left
+                const uint8_t* st = ring + slot;
+                slot = slot == (S::DEPTH - 1) * S::STAGE ? 0 : slot + S::STAGE;
+                uint32_t r[MP][2][4];
+#pragma unroll
+                for (int m = 0; m < 2 * MP; ++m) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(st + m * 512 + lane * 16);
+                    r[m / 2][m & 1][0] = w.x, r[m / 2][m & 1][1] = w.y, r[m / 2][m & 1][2] = w.z, r[m / 2][m & 1][3] = w.w;
+                }
+                const int b = k0 + it * wk - b0;  // in the chunk
+                const __half2* pr = reinterpret_cast<const __half2*>(st + MP * 1024) + i * GB;
+#pragma unroll
+                for (int g = 0; g < GB; ++g) {
+                    float d0[MP][NT][4], d1[MP][NT][4];
+#pragma unroll
+                    for (int n = g * (4 / GB); n < (g + 1) * (4 / GB); ++n) {
+                        uint4 x[NT];
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) x[t] = *reinterpret_cast<const uint4*>(xrow[t] + b * 256 + n * 64);
+#pragma unroll
+                        for (int m = 0; m < MP; ++m) {
+                            constexpr uint32_t ONE = q4::NIBBLES, UP = q4::NIBBLES << 4;
+                            const uint32_t l0 = r[m][0][n], l1 = r[m][1][n], h0 = l0 >> 8, h1 = l1 >> 8;
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) {
+                                if (n == g * (4 / GB)) {
+                                    q4::mma0(d0[m][t], l0 & ONE, l1 & ONE, h0 & ONE, h1 & ONE, x[t].x, x[t].y);
+                                    q4::mma0(d1[m][t], l0 & UP, l1 & UP, h0 & UP, h1 & UP, x[t].z, x[t].w);
+                                } else {
+                                    q4::mma(d0[m][t], l0 & ONE, l1 & ONE, h0 & ONE, h1 & ONE, x[t].x, x[t].y);
+                                    q4::mma(d1[m][t], l0 & UP, l1 & UP, h0 & UP, h1 & UP, x[t].z, x[t].w);
+                                }
+                            }
+                        }
+                    }
+                    float2 xs[NT];
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+                        xs[t] = *reinterpret_cast<const float2*>(xsum + (b * GB + g) * (8 * NT) + 8 * t + 2 * j);
+#pragma unroll
+                    for (int m = 0; m < MP; ++m) {
+                        const float2 p0 = __half22float2(pr[m * 16 * GB + g]), p1 = __half22float2(pr[m * 16 * GB + 8 * GB + g]);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            float(&y)[4] = acc[m][t];
+                            const float(&u)[4] = d0[m][t];
+                            const float(&v)[4] = d1[m][t];
+                            y[0] = fmaf(fmaf(v[0], 0.0625f, u[0]), p0.x, fmaf(xs[t].x, p0.y, y[0]));
+                            y[1] = fmaf(fmaf(v[1], 0.0625f, u[1]), p0.x, fmaf(xs[t].y, p0.y, y[1]));
+                            y[2] = fmaf(fmaf(v[2], 0.0625f, u[2]), p1.x, fmaf(xs[t].x, p1.y, y[2]));
+                            y[3] = fmaf(fmaf(v[3], 0.0625f, u[3]), p1.x, fmaf(xs[t].y, p1.y, y[3]));
                         }
                     }
                 }
-                fetch(u, it + u + W4_AHEAD);
             }
         }
-    }
 
-    // ---- add up the warps of a panel: [warp][token][16 rows]
-    __syncthreads();
-    float* red = reinterpret_cast<float*>(smem);
+        // ---- add up the warps of a unit: [warp][panel][token][16 rows]
+        if (group != static_cast<int>(blockIdx.x)) __syncthreads();  // (the units before have been read)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        float* r = red + (warp * 8 * NT + 8 * t + 2 * j) * 16 + i;
-        r[0] = acc[t][0];
-        r[16] = acc[t][1];
-        r[8] = acc[t][2];
-        r[24] = acc[t][3];
+        for (int m = 0; m < MP; ++m)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float* r = red + ((warp * MP + m) * 8 * NT + 8 * t + 2 * j) * 16 + i;
+                r[0] = acc[m][t][0];
+                r[16] = acc[m][t][1];
+                r[8] = acc[m][t][2];
+                r[24] = acc[m][t][3];
+            }
+        __syncthreads();
+        const int wide_log = 4 + a.wp_log + (MP - 1);  // outputs of the group
+        for (int u = threadIdx.x; u < nt_live << wide_log; u += W4_THREADS) {
+            const int t = u >> wide_log, o = u - (t << wide_log);
+            const int n = (group << wide_log) + o, p = o >> 4;  // panel of the group: warp p / MP, its panel p % MP
+            if (n >= a.out) continue;
+            float y = 0.f;
+            for (int k = 0; k < wk; ++k)
+                y += red[((((k << a.wp_log) + p / MP) * MP + p % MP) * 8 * NT + t) * 16 + (o & 15)];
+            y *= 0x1p24f;
+            if (a.bias) y += __half2float(__ldg(a.bias + n));
+            if (a.act == ET_ACT_RELU) y = fmaxf(y, 0.f);
+            if (a.act == ET_ACT_GELU)
+                y = y * (0.5f + 0.5f * tanhf(y * (0.035677408136300125f * y * y + 0.7978845608028654f)));
+            a.Y[static_cast<int64_t>(t0 + t) * a.out + n] = __float2half_rn(y);
+        }
     }
-    __syncthreads();
-    for (int u = threadIdx.x; u < nt_live * 16 * wp; u += W4_THREADS) {
-        const int t = u / (16 * wp), o = u - t * (16 * wp);
-        const int n = (blockIdx.x * wp) * 16 + o;
-        if (n >= a.out) continue;
-        float y = 0.f;
-        for (int k = 0; k < wk; ++k) y += red[(((k << a.wp_log) + (o >> 4)) * 8 * NT + t) * 16 + (o & 15)];
-        y *= 0x1p24f;
-        if (a.bias) y += __half2float(__ldg(a.bias + n));
-        if (a.act == ET_ACT_RELU) y = fmaxf(y, 0.f);
-        if (a.act == ET_ACT_GELU)
-            y = y * (0.5f + 0.5f * tanhf(y * (0.035677408136300125f * y * y + 0.7978845608028654f)));
-        a.Y[static_cast<int64_t>(t0 + t) * a.out + n] = __float2half_rn(y);
-    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // Sixteen lanes per (row, block of 128 features): lane 4 n + j holds word n of lane j.
@@ -226,43 +304,61 @@ int check_w4(int in, int out, int group) {
     return ET_OK;
 }
 
-template <int GB, int NT>
-int launch_w4(W4Args a, cudaStream_t stream) {
-    auto kern = linear_w4_kernel<GB, NT>;
-    const int rows = a.T < 8 * NT ? a.T : 8 * NT;
-    constexpr int ahead = W4_AHEAD_OF<NT>;
-    const int wk = W4_WARPS >> a.wp_log, unit = wk * ahead;
-    // (16 tokens: 32 blocks a chunk, 132 KB; 32 tokens: 16 blocks, 133 KB)
-    constexpr int most = W4_X_BYTES + 64 * 1024;
-    static_assert(8 * NT * (W4_WARPS * ahead * 256 + 64) <= most, "one chunk fits");
-    auto staged = [&](int blocks) { return static_cast<size_t>(rows) * (static_cast<size_t>(blocks) * 256 + 64); };
-    a.chunk_blocks = (a.nb + unit - 1) / unit * unit;  // all of them, or as many as fit
-    if (staged(a.nb) > W4_X_BYTES || staged(a.chunk_blocks) > static_cast<size_t>(most)) {
-        a.chunk_blocks = (W4_X_BYTES / rows - 64) / 256 / unit * unit;
-        if (a.chunk_blocks < unit) a.chunk_blocks = unit;
-    }
-    size_t smem = staged(a.chunk_blocks);
-    const size_t red = static_cast<size_t>(W4_WARPS) * 8 * NT * 16 * 4;
-    smem = smem > red ? smem : red;
-    if (smem > static_cast<size_t>(most)) return ET_ERR_SHAPE;
+template <int MP, int GB, int NT>
+int launch_w4(W4Args a, int slots, size_t smem, cudaStream_t stream) {
+    auto kern = linear_w4_kernel<MP, GB, NT>;
     static std::atomic<bool> attr_set[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 0 && dev < 64 && !attr_set[dev]) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess)
-            return ET_ERR_CUDA;
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_SMEM) != cudaSuccess) return ET_ERR_CUDA;
         attr_set[dev] = true;
     }
-    const int wp = 1 << a.wp_log;
-    const dim3 grid((a.panels + wp - 1) / wp, (a.T + 8 * NT - 1) / (8 * NT));
+    const int tiles = (a.T + 8 * NT - 1) / (8 * NT), unit = MP << a.wp_log;
+    const int groups = (a.panels + unit - 1) / unit;
+    const int wide = slots / tiles > 1 ? slots / tiles : 1;
+    const dim3 grid(groups < wide ? groups : wide, tiles);
     return launch_kernel(kern, grid, dim3(W4_THREADS), smem, stream, a) == cudaSuccess ? ET_OK : ET_ERR_CUDA;
+}
+
+template <int GB, int NT>
+int plan_w4(W4Args a, cudaStream_t stream) {
+    const int rows = a.T < 8 * NT ? a.T : 8 * NT;
+    const int64_t tiles = (a.T + 8 * NT - 1) / (8 * NT);
+    const int sms = sm_count() > 0 ? sm_count() : 148;
+    using S1 = W4Smem<1, GB, NT>;
+    using S2 = W4Smem<2, GB, NT>;
+    static_assert(S2::RINGS + S2::RED <= S1::RINGS + 2 * S1::RED, "what is left for activations");
+    constexpr size_t fixed = S1::RINGS + 2 * S1::RED;
+    static_assert(W4_SMEM >= 8 * NT * (W4_WARPS * 256 + 64) + W4_WARPS * GB * 8 * NT * 4 + fixed, "one chunk fits");
+    // All activations at once where they fit, else as many blocks as do, a whole number per warp.
+    a.chunk_blocks = (a.nb + W4_WARPS - 1) / W4_WARPS * W4_WARPS;
+    const size_t per_block = static_cast<size_t>(rows) * 256 + GB * 8 * NT * 4;
+    if (a.chunk_blocks * per_block + rows * 64 + fixed > W4_SMEM)
+        a.chunk_blocks = static_cast<int>((W4_SMEM - fixed - rows * 64) / per_block) / W4_WARPS * W4_WARPS;
+    const size_t smem = S1::bytes(rows, a.chunk_blocks), smem2 = S2::bytes(rows, a.chunk_blocks);
+    // The plan that leaves the least for the busiest thread block, counted in panels; of equals the one with the most
+    // outputs side by side (they share staged activations, and two panels a warp its fragments and its loop).
+    int best = 0, mp = 1, slots = sms;
+    for (int m = 1; m <= 2; ++m)
+        for (int w = 0; w <= 2; ++w) {
+            const int places = (NT == 1 && (m == 1 ? smem : smem2) <= 113 * 1024 ? 2 : 1) * sms;
+            const int64_t groups = (a.panels + (m << w) - 1) / (m << w) * tiles;
+            const int cost = static_cast<int>((groups + places - 1) / places) * (m << w) * (places == sms ? 1 : 2);
+            if ((w == 0 && m == 1) || cost <= best) {
+                best = cost;
+                a.wp_log = w;
+                mp = m;
+                slots = places;
+            }
+        }
+    return mp == 1 ? launch_w4<1, GB, NT>(a, slots, smem, stream) : launch_w4<2, GB, NT>(a, slots, smem2, stream);
 }
 
 template <int GB>
 int launch_w4_tokens(const W4Args& a, cudaStream_t stream) {
-    if (a.T <= 8) return launch_w4<GB, 1>(a, stream);
-    if (a.T <= 16) return launch_w4<GB, 2>(a, stream);
-    return launch_w4<GB, 4>(a, stream);
+    if (a.T <= 8) return plan_w4<GB, 1>(a, stream);
+    return plan_w4<GB, 2>(a, stream);
 }
 
 int g_w4_small = -1;  // test hook: -1 = by the token count, 0 = never, 1 = always the kernel for few tokens
@@ -325,7 +421,7 @@ int et_linear_w4_fwd(const uint8_t* codes, const et_half* params, int group, con
     if (act < ET_ACT_NONE || act > ET_ACT_GELU) return ET_ERR_INVALID_ARG;
     const int st = et::check_w4(in, out, group);
     if (st != ET_OK) return st;
-    if (T > 65535 * 32) return ET_ERR_SHAPE;
+    if (T > 65535 * 16) return ET_ERR_SHAPE;
     if (!et::aligned16(codes) || !et::aligned16(params) || !et::aligned16(X) || !et::aligned16(Y))
         return ET_ERR_ALIGNMENT;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -336,7 +432,7 @@ int et_linear_w4_fwd(const uint8_t* codes, const et_half* params, int group, con
                                            reinterpret_cast<const __half*>(X), reinterpret_cast<__half*>(Y), T, in,
                                            out, act, s);
     et::W4Args a = {};
-    a.codes = reinterpret_cast<const uint4*>(codes);
+    a.codes = codes;
     a.params = reinterpret_cast<const __half*>(params);
     a.bias = reinterpret_cast<const __half*>(bias);
     a.X = reinterpret_cast<const __half*>(X);
@@ -344,10 +440,6 @@ int et_linear_w4_fwd(const uint8_t* codes, const et_half* params, int group, con
     a.T = T, a.in = in, a.out = out, a.act = act;
     a.nb = (in + 127) / 128;
     a.panels = out / 16;
-    // Panels per thread block: as many as leave a block for every SM (they share the staged activations).
-    const int sms = et::sm_count() > 0 ? et::sm_count() : 148;
-    a.wp_log = 0;
-    while (a.wp_log < 2 && (a.panels >> (a.wp_log + 1)) >= sms) ++a.wp_log;
     if (group == 128) return et::launch_w4_tokens<1>(a, s);
     if (group == 64) return et::launch_w4_tokens<2>(a, s);
     return et::launch_w4_tokens<4>(a, s);
