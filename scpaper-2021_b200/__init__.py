@@ -360,19 +360,29 @@ def _require(name: str, dtype, *tensors) -> None:
     """Tensors of a call: of one type, on the current device, with contiguous rows."""
     dev = _torch_c()._cuda_getDevice()
     for t in tensors:
-        if t is None:
-            continue
-        if t.dtype is not dtype:
-            raise EtError(f"{name}: a tensor is {t.dtype}, {dtype} is wanted")
-        if not t.is_cuda or t.device.index != dev:
-            raise EtError(f"{name}: a tensor is on {t.device}, the current device is cuda:{dev}")
-        if t.dim() and t.stride(-1) != 1 and t.shape[-1] != 1:
-            raise EtError(f"{name}: the values of a row must be contiguous")
+        if t is not None and (t.dtype is not dtype or t.get_device() != dev or (t.dim() and t.stride(-1) != 1)):
+            if t.dtype is not dtype:
+                raise EtError(f"{name}: a tensor is {t.dtype}, {dtype} is wanted")
+            if t.get_device() != dev:
+                raise EtError(f"{name}: a tensor is on {t.device}, the current device is cuda:{dev}")
+            if t.shape[-1] != 1:
+                raise EtError(f"{name}: the values of a row must be contiguous")
 
 
 def _row_stride(t) -> int:
     """Stride of a matrix's rows (a single row may report any)."""
     return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+_F16 = _I32 = None  # torch's types, once torch is loaded
+
+
+def _types():
+    global _F16, _I32
+    if _F16 is None:
+        import torch
+        _F16, _I32 = torch.float16, torch.int32
+    return _F16, _I32
 
 
 class W4Weight:
@@ -391,6 +401,7 @@ class W4Weight:
         self.params = torch.empty(self.param_shape, dtype=torch.float16, device=w.device)
         _call("et_w4_pack", _a(w), inn, out, group, _a(self.codes), _a(self.params), _raw_stream())
         torch.cuda.current_stream().synchronize()  # weights must be complete before their first use
+        self.codes_at, self.params_at = self.codes.data_ptr(), self.params.data_ptr()
 
     def _set(self, inn: int, out: int, group: int) -> None:
         code_bytes, param_bytes = c_size_t(0), c_size_t(0)
@@ -413,6 +424,7 @@ class W4Weight:
         if not codes.is_contiguous() or not params.is_contiguous():
             raise EtError("W4Weight: contiguous arrays are wanted")
         w.codes, w.params = codes, params
+        w.codes_at, w.params_at = codes.data_ptr(), params.data_ptr()
         return w
 
     def densify(self):
@@ -427,16 +439,22 @@ class W4Weight:
 
 def linear_w4(x, w: "W4Weight", bias=None, act=ACT_NONE, out=None):
     """act(x W^T + bias) with a 4-bit weight; `out`: optional preallocated [T, out] result."""
-    import torch
     T, inn = x.shape
     if inn != w.inn or not x.is_contiguous():
         raise EtError(f"linear_w4: contiguous activations [T, {w.inn}] are wanted")
-    y = _empty((T, w.out), x) if out is None else out
-    _require("linear_w4", torch.float16, x, bias, y)
-    if y.shape != (T, w.out) or not y.is_contiguous() or (bias is not None and bias.shape != (w.out,)):
-        raise EtError(f"linear_w4: out [{T}, {w.out}] and bias [{w.out}] are wanted")
-    _call("et_linear_w4_fwd", _a(w.codes), _a(w.params), w.group, _a(bias), _a(x), _a(y), T, inn, w.out, act,
-          _raw_stream())
+    f16 = _types()[0]
+    if out is None:
+        y = x.new_empty((T, w.out))
+        _require("linear_w4", f16, x, bias)
+    else:
+        y = out
+        _require("linear_w4", f16, x, bias, y)
+        if y.shape != (T, w.out) or not y.is_contiguous():
+            raise EtError(f"linear_w4: a contiguous result [{T}, {w.out}] is wanted")
+    if w.codes.get_device() != x.get_device() or (bias is not None and bias.shape != (w.out,)):
+        raise EtError(f"linear_w4: the weight's device and a bias [{w.out}] are wanted")
+    _call("et_linear_w4_fwd", w.codes_at, w.params_at, w.group, _a(bias), x.data_ptr(), y.data_ptr(), T, inn, w.out,
+          act, _raw_stream())
     return y
 
 
@@ -571,6 +589,8 @@ class KV4Cache:
         self.v_codes, self.v_params = torch.zeros_like(self.k_codes), torch.zeros_like(self.k_params)
         for name in ("k_codes", "k_params", "v_codes", "v_params"):
             setattr(self.desc, name, getattr(self, name).data_ptr())
+        self.device_index = self.k_codes.get_device()
+        self.k_width, self.v_width, self.scale = nkv * dh_qk, nkv * dh_v, 1.0 / dh_qk ** 0.5
         self._at = ctypes.addressof(self.desc)
         self._workspace_bytes = {}
 
@@ -584,48 +604,46 @@ class KV4Cache:
 
 
 def _check_pages(name: str, cache: "KV4Cache", batch: int, table, *lengths) -> None:
-    import torch
-    _require(name, torch.int32, table, *lengths)
-    if cache.k_codes.device != table.device:
+    _require(name, _types()[1], table, *lengths)
+    if cache.device_index != table.get_device():
         raise EtError(f"{name}: the cache is on {cache.k_codes.device}")
     if table.dim() != 2 or table.shape[0] != batch:
         raise EtError(f"{name}: a page table [{batch}, pages] is wanted")
     for n in lengths:
-        if n is not None and n.shape != (batch,):
+        if n is not None and (n.dim() != 1 or n.shape[0] != batch):
             raise EtError(f"{name}: one length per sequence ({batch}) is wanted")
 
 
-def _check_rows(name: str, rows: int, **widths) -> None:
-    for what, (t, width) in widths.items():
-        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width:
-            raise EtError(f"{name}: {what} [{rows}, {width}] is wanted")
+def _check_rows(name: str, what: str, t, rows: int, width: int) -> None:
+    if t.shape != (rows, width):
+        raise EtError(f"{name}: {what} [{rows}, {width}] is wanted")
 
 
 def kv4_write(cache: "KV4Cache", k, v, table, start, batch: int, seq: int, new_len=None) -> None:
     """Quantises k [batch * seq, nkv * dh_qk] and v (views of a fused projection serve) into positions
     start[b] .. of every sequence; rows i >= new_len[b] are padding.  start None: 0."""
-    import torch
-    _require("kv4_write", torch.float16, k, v)
+    _require("kv4_write", _types()[0], k, v)
     _check_pages("kv4_write", cache, batch, table, start, new_len)
-    _check_rows("kv4_write", batch * seq, k=(k, cache.nkv * cache.dh_qk), v=(v, cache.nkv * cache.dh_v))
-    _call("et_kv4_write_fwd", cache._at, _a(k), _a(v), _row_stride(k), _row_stride(v), _a(table),
+    _check_rows("kv4_write", "k", k, batch * seq, cache.k_width)
+    _check_rows("kv4_write", "v", v, batch * seq, cache.v_width)
+    _call("et_kv4_write_fwd", cache._at, k.data_ptr(), v.data_ptr(), _row_stride(k), _row_stride(v), table.data_ptr(),
           _row_stride(table), _a(start), _a(new_len), batch, seq, _raw_stream())
 
 
 def kv4_read(cache: "KV4Cache", table, batch: int, seq: int, start=None, length=None, out=None):
     """(k, v) in fp16 from positions start[b] .. start[b] + length[b] (seq where None) of every sequence;
-    rows behind a sequence's last are left as they were (`out`: a preallocated pair)."""
-    import torch
+    rows behind a sequence's last are left as they were (`out`: a preallocated pair; zeros where None)."""
     _check_pages("kv4_read", cache, batch, table, start, length)
-    rows = batch * seq
+    rows, f16 = batch * seq, _types()[0]
     if out is None:
-        make = torch.empty if length is None else torch.zeros
-        out = tuple(make((rows, cache.nkv * d), dtype=torch.float16, device=table.device)
-                    for d in (cache.dh_qk, cache.dh_v))
-    k, v = out
-    _require("kv4_read", torch.float16, k, v)
-    _check_rows("kv4_read", rows, k=(k, cache.nkv * cache.dh_qk), v=(v, cache.nkv * cache.dh_v))
-    _call("et_kv4_read_fwd", cache._at, _a(k), _a(v), _row_stride(k), _row_stride(v), _a(table),
+        make = table.new_empty if length is None else table.new_zeros
+        k, v = make((rows, cache.k_width), dtype=f16), make((rows, cache.v_width), dtype=f16)
+    else:
+        k, v = out
+        _require("kv4_read", f16, k, v)
+        _check_rows("kv4_read", "k", k, rows, cache.k_width)
+        _check_rows("kv4_read", "v", v, rows, cache.v_width)
+    _call("et_kv4_read_fwd", cache._at, k.data_ptr(), v.data_ptr(), _row_stride(k), _row_stride(v), table.data_ptr(),
           _row_stride(table), _a(start), _a(length), batch, seq, _raw_stream())
     return k, v
 
@@ -635,28 +653,34 @@ def attention_kv4(cache: "KV4Cache", q, table, kv_len, batch: int, seq: int, nhe
     """softmax(q k^T * scale + mask) v of q [batch * seq, nhead * dh_qk] over the kv_len[b] cached tokens of every
     sequence, the queries' own (its newest, written first) included.  max_len: the largest kv_len (the page
     table's reach where None); a tight one lets the call split the sequence well.  q_len[b] < seq: padding rows,
-    left as they were.  mask: fp16 [seq, >= max_len] for MASK_ADDITIVE.  workspace: optional scratch of
-    cache.workspace_bytes(...) bytes, not shared with calls that may overlap."""
-    import torch
+    left as they were (zeros where `out` is None).  mask: fp16 [seq, >= max_len] for MASK_ADDITIVE.  workspace:
+    optional scratch of cache.workspace_bytes(...) bytes, not shared with calls that may overlap."""
     if max_len is None:
         max_len = table.shape[1] * cache.page
-    z = out
-    if z is None:
-        z = (torch.empty if q_len is None else torch.zeros)(
-            (batch * seq, nhead * cache.dh_v), dtype=torch.float16, device=q.device)
-    _require("attention_kv4", torch.float16, q, z, mask)
+    f16, rows = _types()[0], batch * seq
+    _require("attention_kv4", f16, q, out, mask)
     _check_pages("attention_kv4", cache, batch, table, kv_len, q_len)
-    _check_rows("attention_kv4", batch * seq, q=(q, nhead * cache.dh_qk), out=(z, nhead * cache.dh_v))
-    if mask is not None and (mask.dim() != 2 or mask.shape[0] < seq):
-        raise EtError(f"attention_kv4: a mask [{seq}, {max_len}] is wanted")
+    _check_rows("attention_kv4", "q", q, rows, nhead * cache.dh_qk)
+    if out is None:
+        z = (q.new_empty if q_len is None else q.new_zeros)((rows, nhead * cache.dh_v))
+    else:
+        z = out
+        _check_rows("attention_kv4", "out", z, rows, nhead * cache.dh_v)
+    ldm = 0
+    if mask is not None:
+        if mask.dim() != 2 or mask.shape[0] < seq or mask.shape[1] < max_len:
+            raise EtError(f"attention_kv4: a mask [{seq}, {max_len}] is wanted")
+        ldm = _row_stride(mask)
+    n = 0
     if workspace is None:
         n = cache.workspace_bytes(batch, seq, nhead, max_len)
-        workspace = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-    _call("et_attention_kv4_fwd", cache._at, _a(q), _a(z), _a(table), _row_stride(table), _a(kv_len), _a(q_len),
-          batch, seq, nhead, _row_stride(q), _row_stride(z), max_len, mask_kind, _a(mask),
-          0 if mask is None else (_row_stride(mask) if mask.shape[1] >= max_len else mask.shape[1]),
-          (1.0 / cache.dh_qk ** 0.5) if scale is None else scale,
-          _a(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(), _raw_stream())
+        if n:
+            workspace = q.new_empty((n + 1) // 2)
+    else:
+        n = workspace.numel() * workspace.element_size()
+    _call("et_attention_kv4_fwd", cache._at, q.data_ptr(), z.data_ptr(), table.data_ptr(), _row_stride(table),
+          kv_len.data_ptr(), _a(q_len), batch, seq, nhead, _row_stride(q), _row_stride(z), max_len, mask_kind, _a(mask),
+          ldm, cache.scale if scale is None else scale, _a(workspace), n, _raw_stream())
     return z
 
 
@@ -832,10 +856,10 @@ class EncoderLayer:
                        new_len=None):
         """The layer over `seq` new tokens of every sequence at positions start[b] .., the earlier ones in
         `cache` (this layer's own); kv_len = start + new_len."""
-        import torch
-        _require("forward_cached", torch.float16, x, out)
+        _require("forward_cached", _types()[0], x, out)
         _check_pages("forward_cached", cache, batch, table, start, kv_len, new_len)
-        _check_rows("forward_cached", batch * seq, x=(x, self.hidden), out=(out, self.hidden))
+        _check_rows("forward_cached", "x", x, batch * seq, self.hidden)
+        _check_rows("forward_cached", "out", out, batch * seq, self.hidden)
         if not x.is_contiguous() or not out.is_contiguous():
             raise EtError("forward_cached: contiguous x and out are wanted")
         _call("et_encoder_layer_cached_fwd", ctypes.addressof(self.desc), cache._at, _a(x), _a(out), batch, seq,

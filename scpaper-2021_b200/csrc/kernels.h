@@ -98,6 +98,7 @@ int launch_linear_expand_packed(const uint32_t* pk_mask, const int* pk_off, cons
 // linear_expand.cu.  Arguments already checked.
 int launch_linear_expand_w4(const uint8_t* codes, const __half* params, int group, const __half* bias,
                             const __half* X, __half* Y, int T, int in, int out, int act, cudaStream_t stream);
+double linear_expand_w4_us(int T, int in, int out);  // its expected time
 
 // Fused attention (see attention.cu).  row_per_thread = false keeps every head width on the kernel whose
 // body attention_fuse_o.cu shares, so that the two give the same bits.

@@ -31,6 +31,8 @@ enum : int { FMT_VEC = 0, FMT_PACKED = 1, FMT_CSRM = 2, FMT_QUANT = 3 };
 
 constexpr int X_MAX_A = 8;                       // activation stages at most
 constexpr int X_MAX_B = 4;                       // weight buffers at most
+constexpr int X_QUANT_B = 2;                     // 4 bits: weight buffers, twice as large,
+constexpr int X_QUANT_A = 6;                     // and activation stages
 constexpr int X_MAX_MB = 8;                      // token blocks per CTA at most
 constexpr int X_CSR_A = 4;                       // CSR: activation stages,
 constexpr int X_CSR_BYTES = 128 * 1024;          // and bytes of expanded columns at most
@@ -178,77 +180,85 @@ struct PackedExpander {
     }
 };
 
-// The same for 4-bit codes: every element of the 16 rows is written.  A code becomes fp16 exactly (1024 + c,
-// less 1024), and c s + m is rounded to fp16 once: the tensor core cannot scale its sums per group, so the
-// operand has to carry the scale.  Lane 4 i + j expands words 2 q and 2 q + 1 (q: which half of the 128-feature
-// block) of rows i and i + 8, fetched QUANT_AHEAD items ahead (with one, 33 tokens x 8192 -> 8192 took 48 us: a trip to
-// memory per item).
+// The same for 4-bit codes, a whole block of 16 rows x 128 features (two K blocks) at a time: every element is
+// written.  A code becomes fp16 exactly (1024 + c, less 1024), and c s + m is rounded to fp16 once: the tensor
+// core cannot scale its sums per group, so the operand has to carry the scale.  Lane 4 i + j expands the four
+// words of rows i and i + 8.  Blocks are copied asynchronously QUANT_AHEAD ahead into a ring of the warp's own (loads into
+// registers are waited for together with younger ones: 64 tokens x 8192 -> 8192 took 33 us).
 constexpr int QUANT_AHEAD = 4;
+constexpr int QUANT_BLOCK = 1024 + 256;  // codes, and (s, m) of 16 rows x up to four groups
 struct QuantExpander {
-    struct Item {
-        uint2 v[2];
-        uint32_t sm[2][2];  // [row half][word]
-    } q[QUANT_AHEAD];
-    const uint2* codes;      // of the next item to fetch
-    const uint32_t* params;
-    int next, nkb, gb, lane, step;
+    uint32_t ring32;
+    const uint8_t* ring;
+    const uint8_t* codes;  // of the next block to fetch
+    const uint8_t* params;
+    int next, nb, gb_log, lane, step;
 
-    __device__ __forceinline__ void fetch(Item& x) {
-        if (next < nkb) {
-            const int h2 = next & 1;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                x.v[h] = __ldg(codes + h * 64 + h2);
-                x.sm[h][0] = __ldg(params + h * 8 * gb + ((2 * h2 * gb) >> 2));
-                x.sm[h][1] = __ldg(params + h * 8 * gb + (((2 * h2 + 1) * gb) >> 2));
-            }
-            // the block of the next item: (step + the item's own half) / 2 further on
-            const int blocks = (h2 + step) >> 1;
-            codes += blocks * 128;
-            params += blocks * 16 * gb;
+    __device__ __forceinline__ void fetch(int slot) {
+        if (next < nb) {
+            const uint32_t to = ring32 + slot * QUANT_BLOCK + lane * 16;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(codes) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 512), "l"(codes + 512) : "memory");
+            if (lane < 4 << gb_log)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 1024), "l"(params) : "memory");
+            codes += step * 1024;
+            params += (step * 64) << gb_log;
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
         next += step;
     }
-    __device__ __forceinline__ void init(const ExpandArgs& a, int panel, int lane_) {
+    __device__ __forceinline__ void start(const ExpandArgs& a, int panel, int first, int step_, int lane_, uint8_t* ring_) {
         lane = lane_;
-        const int nb = (a.in + 127) >> 7;
-        nkb = (a.in + BK - 1) / BK;
-        gb = 128 / a.group;
-        codes = reinterpret_cast<const uint2*>(a.data) + static_cast<size_t>(panel) * nb * 128 + lane * 2;
-        params = reinterpret_cast<const uint32_t*>(a.idx0) + static_cast<size_t>(panel) * nb * 16 * gb + (lane >> 2) * gb;
-    }
-    __device__ __forceinline__ void start(int kb, int step_) {
+        nb = (a.in + 127) >> 7;
+        gb_log = a.group == 128 ? 0 : (a.group == 64 ? 1 : 2);  // groups per block
         step = step_;
-        next = kb;
-        codes += (kb >> 1) * 128;
-        params += (kb >> 1) * 16 * gb;
+        next = first;
+        ring = ring_;
+        ring32 = smem_u32(ring_);
+        const size_t at = static_cast<size_t>(panel) * nb + first;
+        codes = reinterpret_cast<const uint8_t*>(a.data) + at * 1024 + lane * 16;
+        params = reinterpret_cast<const uint8_t*>(a.idx0) + ((at * 64) << gb_log) + lane * 16;
 #pragma unroll
-        for (int u = 0; u < QUANT_AHEAD; ++u) fetch(q[u]);
+        for (int u = 0; u < QUANT_AHEAD; ++u) fetch(u);
     }
-    // expands one item of the ring into `tile` and fills its place again
-    __device__ __forceinline__ void write(uint8_t* tile, Item& x) {
+    // expands the ring's block `slot` into the rows at `tile` and, `next_kb` bytes on, of the next K block; its place
+    // is filled again
+    __device__ __forceinline__ void write(uint8_t* tile, int next_kb, int slot) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(QUANT_AHEAD - 1) : "memory");
+        __syncwarp();
+        const uint8_t* at = ring + slot * QUANT_BLOCK;
+        uint4 v[2];
+        uint32_t sm[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            v[h] = *reinterpret_cast<const uint4*>(at + h * 512 + lane * 16);
+            const uint32_t* p = reinterpret_cast<const uint32_t*>(at + 1024) + ((8 * h + (lane >> 2)) << gb_log);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) sm[h][n] = p[(n << gb_log) >> 2];
+        }
+        __syncwarp();
+        fetch(slot);
         const __half2 base = __floats2half2_rn(1024.f, 1024.f);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int row = 8 * h + (lane >> 2), j = lane & 3;
             uint8_t* line = tile + row * 128;
+            const uint32_t words[4] = {v[h].x, v[h].y, v[h].z, v[h].w};
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const uint32_t w = n ? x.v[h].y : x.v[h].x;
-                const __half2 pair = *reinterpret_cast<const __half2*>(&x.sm[h][n]);
+            for (int n = 0; n < 4; ++n) {
+                const __half2 pair = *reinterpret_cast<const __half2*>(&sm[h][n]);
                 const __half2 s = __low2half2(pair), m = __high2half2(pair);
                 uint32_t o[4];
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
-                    const uint32_t c = q4::and_or(w >> (4 * p), q4::NIBBLES, 0x64006400u);
+                    const uint32_t c = q4::and_or(words[n] >> (4 * p), q4::NIBBLES, 0x64006400u);
                     const __half2 y = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), base), s, m);
                     o[p] = *reinterpret_cast<const uint32_t*>(&y);
                 }
-                *reinterpret_cast<uint4*>(line + (((n * 4 + j) ^ (row & 7)) * 16)) =
+                *reinterpret_cast<uint4*>(line + (n >> 1) * next_kb + ((((n & 1) * 4 + j) ^ (row & 7)) * 16)) =
                     make_uint4(o[0], o[1], o[2], o[3]);
             }
         }
-        fetch(x);
     }
 };
 
@@ -312,6 +322,7 @@ linear_expand_kernel(const __grid_constant__ CUtensorMap tmX, const ExpandArgs g
     float* s_bias = reinterpret_cast<float*>(misc + 256);         // [BN]
     int* s_ptr = reinterpret_cast<int*>(s_bias + BN);             // CSR: [BN + 1] row starts
     int* s_dup = s_ptr + X_ROW_LIST;                              // CSR: [BN] row holds duplicates
+    uint8_t* s_ring = reinterpret_cast<uint8_t*>(s_bias + BN);    // 4 bits: the expanding warps' rings
 
     const int warp = uniform_warp_id();
     const int lane = threadIdx.x & 31;
@@ -493,30 +504,28 @@ linear_expand_kernel(const __grid_constant__ CUtensorMap tmX, const ExpandArgs g
                 if (lane == 0) mbar_arrive(&b_full[buf]);
             }
         } else if constexpr (FMT == FMT_QUANT) {
-            // As below, by four items a round, whose registers the compiler then knows by name.
+            // Item (16 output rows, block of 128 features) of a buffer per warp: BN / 16 row sets x ckb / 2 blocks = 8,
+            // QUANT_AHEAD buffers a round.
             constexpr int SETS = BN / 16;
             const int set = w % SETS, sub = w / SETS;
             const bool live = n0 + set * 16 < g.out;
             QuantExpander x;
-            if (live) {
-                x.init(g, (n0 >> 4) + set, lane);
-                x.start(sub, g.ckb);
-            }
-            static_assert(X_MAX_B == QUANT_AHEAD, "a round fills every buffer once");
-            uint32_t bph = 0;
-            for (int c0 = 0; c0 < nchunk; c0 += QUANT_AHEAD, bph ^= 1u)
+            if (live) x.start(g, (n0 >> 4) + set, sub, g.ckb >> 1, lane, s_ring + w * (QUANT_AHEAD * QUANT_BLOCK));
+            static_assert(QUANT_AHEAD % (2 * X_QUANT_B) == 0, "buffers and their parities repeat every round");
+            for (int c0 = 0; c0 < nchunk; c0 += QUANT_AHEAD)
 #pragma unroll
                 for (int u = 0; u < QUANT_AHEAD; ++u) {
                     if (c0 + u >= nchunk) break;
+                    constexpr int NB = X_QUANT_B;
                     if (ok) {
-                        ok = mbar_wait_bounded(&b_empty[u], bph ^ 1, abort_flag);
+                        ok = mbar_wait_bounded(&b_empty[u % NB], ((u / NB) & 1) ^ 1, abort_flag);
                         ok = __all_sync(0xffffffffu, ok);
                     }
-                    uint8_t* tile = sB + u * buf_bytes + sub * (BN * 128) + set * (16 * 128);
-                    if (live && (c0 + u) * g.ckb + sub < nkb) x.write(tile, x.q[u]);
+                    uint8_t* tile = sB + (u % NB) * buf_bytes + 2 * sub * (BN * 128) + set * (16 * 128);
+                    if (live && ((c0 + u) * g.ckb >> 1) + sub < x.nb) x.write(tile, BN * 128, u);
                     fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&b_full[u]);
+                    if (lane == 0) mbar_arrive(&b_full[u % NB]);
                 }
         } else {
             // Item (16 output rows, K block) of a buffer per warp: BN / 16 row sets x ckb blocks = 8.
@@ -649,13 +658,15 @@ linear_expand_kernel(const __grid_constant__ CUtensorMap tmX, const ExpandArgs g
 template <int FMT, int BN>
 int launch_bn(const CUtensorMap& tmX, ExpandArgs& a, cudaStream_t stream) {
     const int buf = a.ckb * BN * 128;
-    constexpr int misc = 256 + BN * 4 + (FMT == FMT_CSRM ? (X_ROW_LIST + BN) * 4 : 0);
+    constexpr int misc = 256 + BN * 4 + (FMT == FMT_CSRM ? (X_ROW_LIST + BN) * 4 : 0) +
+                         (FMT == FMT_QUANT ? X_EXP_WARPS * QUANT_AHEAD * QUANT_BLOCK : 0);
     const int smem = a.na * A_STAGE_BYTES + a.nbuf * buf + misc + 1024;
     auto kern = linear_expand_kernel<FMT, BN>;
     // once, to the most that any width needs: two threads that each raised it to their own size could leave
     // the smaller one standing
     constexpr int most = (FMT == FMT_CSRM ? X_CSR_A * A_STAGE_BYTES + X_CSR_BYTES
-                                          : X_MAX_A * A_STAGE_BYTES + X_MAX_B * 128 * 128) + misc + 1024;
+                                          : (FMT == FMT_QUANT ? X_QUANT_A : X_MAX_A) * A_STAGE_BYTES +
+                                                X_MAX_B * 128 * 128) + misc + 1024;
     static_assert(most <= 227 * 1024, "shared memory budget exceeded");
     static std::atomic<bool> attr_set[64] = {};
     int dev = 0;
@@ -710,6 +721,10 @@ ExpandPlan plan_expand(ExpandArgs& a) {
         a.ckb = nkb < fit ? nkb : fit;
         a.nbuf = 1;
         a.na = X_CSR_A;
+    } else if (FMT == FMT_QUANT) {
+        a.ckb = 256 / bn;  // eight warps, one (row set, two K blocks) item each
+        a.nbuf = X_QUANT_B;
+        a.na = X_QUANT_A;
     } else {
         a.ckb = 128 / bn;  // eight warps, one (row set, K block) item each
         a.nbuf = X_MAX_B;
@@ -772,6 +787,17 @@ int launch_linear_expand_packed(const uint32_t* pk_mask, const int* pk_off, cons
     a.out = out;
     a.act = act;
     return launch_expand<FMT_PACKED>(a, stream);
+}
+
+// Every K block of a CTA's token block costs one thread four products and their completion, 0.24 us whatever the
+// panel's width.
+double linear_expand_w4_us(int T, int in, int out) {
+    ExpandArgs a = {};
+    a.T = T;
+    a.in = in;
+    a.out = out;
+    const ExpandPlan p = plan_expand<FMT_QUANT>(a);
+    return 1.7 + 0.24 * ((in + BK - 1) / BK) * p.waves * a.mb;
 }
 
 int launch_linear_expand_w4(const uint8_t* codes, const __half* params, int group, const __half* bias,

@@ -42,34 +42,34 @@ __device__ __forceinline__ void w4_copy16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-// MP panels of 16 rows to a warp, GB groups per block of 128 features, NT tiles of eight tokens.
-// Shared memory: activations [rows][chunk + 64 bytes], their sums [chunk groups][8 NT], the warps' sums, the rings.
+// MP panels of 16 rows to a warp, GB groups per block of 128 features; eight tokens.
+// Shared memory: activations [rows][chunk + 64 bytes], their sums [chunk groups][8], the warps' sums, the rings.
 // (Activation rows lie 64 bytes apart in the banks: eight lanes - two tokens, four pieces - meet no conflict.)
-template <int MP, int GB, int NT>
+template <int MP, int GB>
 struct W4Smem {
     static constexpr int DEPTH = MP == 2 ? 4 : 8;  // stages of a ring, of 2 or 1 KB of codes
     static constexpr int STAGE = MP * (1024 + 64 * GB);
     static constexpr int RINGS = W4_WARPS * DEPTH * STAGE;
-    static constexpr int RED = W4_WARPS * MP * 8 * NT * 16 * 4;
+    static constexpr int RED = W4_WARPS * MP * 8 * 16 * 4;
     static size_t bytes(int rows, int chunk) {
-        return static_cast<size_t>(rows) * (chunk * 256 + 64) + static_cast<size_t>(chunk) * GB * 8 * NT * 4 + RED + RINGS;
+        return static_cast<size_t>(rows) * (chunk * 256 + 64) + static_cast<size_t>(chunk) * GB * 8 * 4 + RED + RINGS;
     }
 };
 
-template <int MP, int GB, int NT>
-__global__ void __launch_bounds__(W4_THREADS, NT == 1 ? 2 : 1) linear_w4_kernel(const W4Args a) {
-    using S = W4Smem<MP, GB, NT>;
+template <int MP, int GB>
+__global__ void __launch_bounds__(W4_THREADS, 2) linear_w4_kernel(const W4Args a) {
+    using S = W4Smem<MP, GB>;
     extern __shared__ __align__(16) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int i = lane >> 2, j = lane & 3;
     const int wp = 1 << a.wp_log, wk = W4_WARPS >> a.wp_log;
     const int k0 = warp >> a.wp_log, w0 = warp & (wp - 1);
-    const int t0 = blockIdx.y * 8 * NT;
-    const int nt_live = a.T - t0 < 8 * NT ? a.T - t0 : 8 * NT;
-    const int rows = a.T < 8 * NT ? a.T : 8 * NT;
+    const int t0 = blockIdx.y * 8;
+    const int nt_live = a.T - t0 < 8 ? a.T - t0 : 8;
+    const int rows = a.T < 8 ? a.T : 8;
     const int ldx = a.chunk_blocks * 256 + 64;
     float* xsum = reinterpret_cast<float*>(smem + rows * ldx);
-    float* red = xsum + a.chunk_blocks * GB * 8 * NT;
+    float* red = xsum + a.chunk_blocks * GB * 8;
     uint8_t* ring = reinterpret_cast<uint8_t*>(red) + S::RED + warp * (S::DEPTH * S::STAGE);
 
     // ---- the warp's blocks, in order: k0, k0 + wk, ... of units (MP panels) w0, w0 + wp grid, ...
@@ -117,14 +117,13 @@ __global__ void __launch_bounds__(W4_THREADS, NT == 1 ? 2 : 1) linear_w4_kernel(
 
     int slot = 0;
     const int per_chunk = a.chunk_blocks / wk;  // of a warp
-    uint8_t* xrow[NT];                          // the lane's tokens; past the last, that one again (never stored)
-#pragma unroll
-    for (int t = 0; t < NT; ++t) xrow[t] = smem + (8 * t + i < nt_live ? 8 * t + i : nt_live - 1) * ldx + j * 16;
+    // the lane's token; past the last, that one again (never stored)
+    uint8_t* xrow = smem + (i < nt_live ? i : nt_live - 1) * ldx + j * 16;
     for (int group = blockIdx.x; group < groups; group += gridDim.x) {
         const bool live = group * wp + w0 < units;
-        float acc[MP][NT][4];
+        float acc[MP][4];
 #pragma unroll
-        for (int k = 0; k < MP * NT * 4; ++k) acc[k / (4 * NT)][k / 4 % NT][k % 4] = 0.f;
+        for (int k = 0; k < MP * 4; ++k) acc[k / 4][k % 4] = 0.f;
         for (int c = 0, b0 = 0; b0 < a.nb; ++c, b0 += a.chunk_blocks) {
             // ---- stage activations and their sums over groups (once, if they fit whole)
             // With one unit at a time a warp reads no features but those of its own blocks, and stages them alone.
@@ -151,23 +150,20 @@ __global__ void __launch_bounds__(W4_THREADS, NT == 1 ? 2 : 1) linear_w4_kernel(
                 else __syncwarp();
                 for (int b = warp; b < blocks; b += W4_WARPS) {
 #pragma unroll
-                    for (int g = 0; g < GB; ++g)
+                    for (int g = 0; g < GB; ++g) {
+                        float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                            for (int n = g * (4 / GB); n < (g + 1) * (4 / GB); ++n) {
-                                uint4* at = reinterpret_cast<uint4*>(xrow[t] + b * 256 + n * 64);
-                                const uint4 x = *at;
-                                q4::mma(d, W4_ONES, W4_ONES, W4_ONES, W4_ONES, x.x, x.y);
-                                q4::mma(d, W4_ONES, W4_ONES, W4_ONES, W4_ONES, x.z, x.w);
-                                // pairs 0 and 2, 1 and 3 together: the second operand's registers below
-                                if (8 * t + i < nt_live) *at = make_uint4(x.x, x.z, x.y, x.w);
-                            }
-                            if (i == 0)
-                                *reinterpret_cast<float2*>(xsum + (b * GB + g) * (8 * NT) + 8 * t + 2 * j) =
-                                    make_float2(d[0], d[1]);
+                        for (int n = g * (4 / GB); n < (g + 1) * (4 / GB); ++n) {
+                            uint4* at = reinterpret_cast<uint4*>(xrow + b * 256 + n * 64);
+                            const uint4 v = *at;
+                            q4::mma(d, W4_ONES, W4_ONES, W4_ONES, W4_ONES, v.x, v.y);
+                            q4::mma(d, W4_ONES, W4_ONES, W4_ONES, W4_ONES, v.z, v.w);
+                            // pairs 0 and 2, 1 and 3 together: the second operand's registers below
+                            if (i < nt_live) *at = make_uint4(v.x, v.z, v.y, v.w);
                         }
+                        if (i == 0)
+                            *reinterpret_cast<float2*>(xsum + (b * GB + g) * 8 + 2 * j) = make_float2(d[0], d[1]);
+                    }
                 }
                 if (wp > 1) __syncthreads();
                 else __syncwarp();
@@ -189,45 +185,31 @@ __global__ void __launch_bounds__(W4_THREADS, NT == 1 ? 2 : 1) linear_w4_kernel(
                 const __half2* pr = reinterpret_cast<const __half2*>(st + MP * 1024) + i * GB;
 #pragma unroll
                 for (int g = 0; g < GB; ++g) {
-                    float d0[MP][NT][4], d1[MP][NT][4];
+                    float d0[MP][4], d1[MP][4];
 #pragma unroll
                     for (int n = g * (4 / GB); n < (g + 1) * (4 / GB); ++n) {
-                        uint4 x[NT];
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) x[t] = *reinterpret_cast<const uint4*>(xrow[t] + b * 256 + n * 64);
+                        const uint4 x = *reinterpret_cast<const uint4*>(xrow + b * 256 + n * 64);
 #pragma unroll
                         for (int m = 0; m < MP; ++m) {
                             constexpr uint32_t ONE = q4::NIBBLES, UP = q4::NIBBLES << 4;
                             const uint32_t l0 = r[m][0][n], l1 = r[m][1][n], h0 = l0 >> 8, h1 = l1 >> 8;
-#pragma unroll
-                            for (int t = 0; t < NT; ++t) {
-                                if (n == g * (4 / GB)) {
-                                    q4::mma0(d0[m][t], l0 & ONE, l1 & ONE, h0 & ONE, h1 & ONE, x[t].x, x[t].y);
-                                    q4::mma0(d1[m][t], l0 & UP, l1 & UP, h0 & UP, h1 & UP, x[t].z, x[t].w);
-                                } else {
-                                    q4::mma(d0[m][t], l0 & ONE, l1 & ONE, h0 & ONE, h1 & ONE, x[t].x, x[t].y);
-                                    q4::mma(d1[m][t], l0 & UP, l1 & UP, h0 & UP, h1 & UP, x[t].z, x[t].w);
-                                }
+                            if (n == g * (4 / GB)) {
+                                q4::mma0(d0[m], l0 & ONE, l1 & ONE, h0 & ONE, h1 & ONE, x.x, x.y);
+                                q4::mma0(d1[m], l0 & UP, l1 & UP, h0 & UP, h1 & UP, x.z, x.w);
+                            } else {
+                                q4::mma(d0[m], l0 & ONE, l1 & ONE, h0 & ONE, h1 & ONE, x.x, x.y);
+                                q4::mma(d1[m], l0 & UP, l1 & UP, h0 & UP, h1 & UP, x.z, x.w);
                             }
                         }
                     }
-                    float2 xs[NT];
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-                        xs[t] = *reinterpret_cast<const float2*>(xsum + (b * GB + g) * (8 * NT) + 8 * t + 2 * j);
+                    const float2 xs = *reinterpret_cast<const float2*>(xsum + (b * GB + g) * 8 + 2 * j);
 #pragma unroll
                     for (int m = 0; m < MP; ++m) {
                         const float2 p0 = __half22float2(pr[m * 16 * GB + g]), p1 = __half22float2(pr[m * 16 * GB + 8 * GB + g]);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            float(&y)[4] = acc[m][t];
-                            const float(&u)[4] = d0[m][t];
-                            const float(&v)[4] = d1[m][t];
-                            y[0] = fmaf(fmaf(v[0], 0.0625f, u[0]), p0.x, fmaf(xs[t].x, p0.y, y[0]));
-                            y[1] = fmaf(fmaf(v[1], 0.0625f, u[1]), p0.x, fmaf(xs[t].y, p0.y, y[1]));
-                            y[2] = fmaf(fmaf(v[2], 0.0625f, u[2]), p1.x, fmaf(xs[t].x, p1.y, y[2]));
-                            y[3] = fmaf(fmaf(v[3], 0.0625f, u[3]), p1.x, fmaf(xs[t].y, p1.y, y[3]));
-                        }
+                        acc[m][0] = fmaf(fmaf(d1[m][0], 0.0625f, d0[m][0]), p0.x, fmaf(xs.x, p0.y, acc[m][0]));
+                        acc[m][1] = fmaf(fmaf(d1[m][1], 0.0625f, d0[m][1]), p0.x, fmaf(xs.y, p0.y, acc[m][1]));
+                        acc[m][2] = fmaf(fmaf(d1[m][2], 0.0625f, d0[m][2]), p1.x, fmaf(xs.x, p1.y, acc[m][2]));
+                        acc[m][3] = fmaf(fmaf(d1[m][3], 0.0625f, d0[m][3]), p1.x, fmaf(xs.y, p1.y, acc[m][3]));
                     }
                 }
             }
@@ -236,15 +218,13 @@ __global__ void __launch_bounds__(W4_THREADS, NT == 1 ? 2 : 1) linear_w4_kernel(
         // ---- add up the warps of a unit: [warp][panel][token][16 rows]
         if (group != static_cast<int>(blockIdx.x)) __syncthreads();  // (the units before have been read)
 #pragma unroll
-        for (int m = 0; m < MP; ++m)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                float* r = red + ((warp * MP + m) * 8 * NT + 8 * t + 2 * j) * 16 + i;
-                r[0] = acc[m][t][0];
-                r[16] = acc[m][t][1];
-                r[8] = acc[m][t][2];
-                r[24] = acc[m][t][3];
-            }
+        for (int m = 0; m < MP; ++m) {
+            float* r = red + ((warp * MP + m) * 8 + 2 * j) * 16 + i;
+            r[0] = acc[m][0];
+            r[16] = acc[m][1];
+            r[8] = acc[m][2];
+            r[24] = acc[m][3];
+        }
         __syncthreads();
         const int wide_log = 4 + a.wp_log + (MP - 1);  // outputs of the group
         for (int u = threadIdx.x; u < nt_live << wide_log; u += W4_THREADS) {
@@ -253,7 +233,7 @@ __global__ void __launch_bounds__(W4_THREADS, NT == 1 ? 2 : 1) linear_w4_kernel(
             if (n >= a.out) continue;
             float y = 0.f;
             for (int k = 0; k < wk; ++k)
-                y += red[((((k << a.wp_log) + p / MP) * MP + p % MP) * 8 * NT + t) * 16 + (o & 15)];
+                y += red[((((k << a.wp_log) + p / MP) * MP + p % MP) * 8 + t) * 16 + (o & 15)];
             y *= 0x1p24f;
             if (a.bias) y += __half2float(__ldg(a.bias + n));
             if (a.act == ET_ACT_RELU) y = fmaxf(y, 0.f);
@@ -304,9 +284,9 @@ int check_w4(int in, int out, int group) {
     return ET_OK;
 }
 
-template <int MP, int GB, int NT>
+template <int MP, int GB>
 int launch_w4(W4Args a, int slots, size_t smem, cudaStream_t stream) {
-    auto kern = linear_w4_kernel<MP, GB, NT>;
+    auto kern = linear_w4_kernel<MP, GB>;
     static std::atomic<bool> attr_set[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
@@ -314,26 +294,26 @@ int launch_w4(W4Args a, int slots, size_t smem, cudaStream_t stream) {
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, W4_SMEM) != cudaSuccess) return ET_ERR_CUDA;
         attr_set[dev] = true;
     }
-    const int tiles = (a.T + 8 * NT - 1) / (8 * NT), unit = MP << a.wp_log;
+    const int tiles = (a.T + 8 - 1) / (8), unit = MP << a.wp_log;
     const int groups = (a.panels + unit - 1) / unit;
     const int wide = slots / tiles > 1 ? slots / tiles : 1;
     const dim3 grid(groups < wide ? groups : wide, tiles);
     return launch_kernel(kern, grid, dim3(W4_THREADS), smem, stream, a) == cudaSuccess ? ET_OK : ET_ERR_CUDA;
 }
 
-template <int GB, int NT>
+template <int GB>
 int plan_w4(W4Args a, cudaStream_t stream) {
-    const int rows = a.T < 8 * NT ? a.T : 8 * NT;
-    const int64_t tiles = (a.T + 8 * NT - 1) / (8 * NT);
+    const int rows = a.T < 8 ? a.T : 8;
+    const int64_t tiles = (a.T + 8 - 1) / (8);
     const int sms = sm_count() > 0 ? sm_count() : 148;
-    using S1 = W4Smem<1, GB, NT>;
-    using S2 = W4Smem<2, GB, NT>;
+    using S1 = W4Smem<1, GB>;
+    using S2 = W4Smem<2, GB>;
     static_assert(S2::RINGS + S2::RED <= S1::RINGS + 2 * S1::RED, "what is left for activations");
     constexpr size_t fixed = S1::RINGS + 2 * S1::RED;
-    static_assert(W4_SMEM >= 8 * NT * (W4_WARPS * 256 + 64) + W4_WARPS * GB * 8 * NT * 4 + fixed, "one chunk fits");
+    static_assert(W4_SMEM >= 8 * (W4_WARPS * 256 + 64) + W4_WARPS * GB * 8 * 4 + fixed, "one chunk fits");
     // All activations at once where they fit, else as many blocks as do, a whole number per warp.
     a.chunk_blocks = (a.nb + W4_WARPS - 1) / W4_WARPS * W4_WARPS;
-    const size_t per_block = static_cast<size_t>(rows) * 256 + GB * 8 * NT * 4;
+    const size_t per_block = static_cast<size_t>(rows) * 256 + GB * 8 * 4;
     if (a.chunk_blocks * per_block + rows * 64 + fixed > W4_SMEM)
         a.chunk_blocks = static_cast<int>((W4_SMEM - fixed - rows * 64) / per_block) / W4_WARPS * W4_WARPS;
     const size_t smem = S1::bytes(rows, a.chunk_blocks), smem2 = S2::bytes(rows, a.chunk_blocks);
@@ -342,7 +322,7 @@ int plan_w4(W4Args a, cudaStream_t stream) {
     int best = 0, mp = 1, slots = sms;
     for (int m = 1; m <= 2; ++m)
         for (int w = 0; w <= 2; ++w) {
-            const int places = (NT == 1 && (m == 1 ? smem : smem2) <= 113 * 1024 ? 2 : 1) * sms;
+            const int places = ((m == 1 ? smem : smem2) <= 113 * 1024 ? 2 : 1) * sms;
             const int64_t groups = (a.panels + (m << w) - 1) / (m << w) * tiles;
             const int cost = static_cast<int>((groups + places - 1) / places) * (m << w) * (places == sms ? 1 : 2);
             if ((w == 0 && m == 1) || cost <= best) {
@@ -352,17 +332,22 @@ int plan_w4(W4Args a, cudaStream_t stream) {
                 slots = places;
             }
         }
-    return mp == 1 ? launch_w4<1, GB, NT>(a, slots, smem, stream) : launch_w4<2, GB, NT>(a, slots, smem2, stream);
+    return mp == 1 ? launch_w4<1, GB>(a, slots, smem, stream) : launch_w4<2, GB>(a, slots, smem2, stream);
 }
 
-template <int GB>
-int launch_w4_tokens(const W4Args& a, cudaStream_t stream) {
-    if (a.T <= 8) return plan_w4<GB, 1>(a, stream);
-    return plan_w4<GB, 2>(a, stream);
+// Whether this kernel, eight tokens at a time, is expected to be faster than expanding the weights to operand
+// tiles, which costs the same for 128 tokens as for one (linear_expand.cu).  Its time is 3 us and 0.32 ns for
+// each block of 16 x 128 weights and eight tokens, fitted to B200 runs; this / expanding in us: 8192 -> 8192 at 8 tokens
+// 12.6 / 32.0, 32 tokens 32.7 / 32.2, 64 tokens 61.9 / 32.1; 4096 -> 1024 at 64 tokens 7.5 / 15.3, 128 tokens 14.8 / 15.4;
+// 1024 -> 4096 at 32 tokens 5.2 / 7.4, 64 tokens 8.9 / 5.8; 768 -> 2304 at 64 tokens 4.7 / 4.5; 512 -> 512 at 128
+// tokens 3.5 / 3.6.
+int g_w4_few = -1;  // test hook: -1 = automatic, 0 = never, 1 = always
+bool w4_few_pay(int T, int in, int out) {
+    if (T > 65535 * 8) return false;  // (its grid)
+    if (g_w4_few >= 0) return g_w4_few != 0;
+    const double blocks = static_cast<double>((in + 127) / 128) * (out / 16) * ((T + 7) / 8);
+    return 3.0 + 0.00032 * blocks < linear_expand_w4_us(T, in, out) || T <= 8;
 }
-
-int g_w4_small = -1;  // test hook: -1 = by the token count, 0 = never, 1 = always the kernel for few tokens
-constexpr int W4_SMALL_T = 32;
 
 }  // namespace
 }  // namespace et
@@ -370,7 +355,10 @@ constexpr int W4_SMALL_T = 32;
 extern "C" {
 
 #ifdef ET_TEST_HOOKS
-void et_debug_set_w4_small(int mode) { et::g_w4_small = mode; }
+// Test hook: the kernel for few tokens: -1 = automatic, 0 = never, 1 = always.
+void et_debug_set_w4_few(int mode) { et::g_w4_few = mode; }
+// Test hook: 1 when that kernel is chosen for the size.
+int et_debug_w4_few_pay(int T, int in, int out) { return et::w4_few_pay(T, in, out) ? 1 : 0; }
 #endif  // ET_TEST_HOOKS
 
 int et_w4_sizes(int in, int out, int group, size_t* code_bytes, size_t* param_bytes) {
@@ -421,12 +409,11 @@ int et_linear_w4_fwd(const uint8_t* codes, const et_half* params, int group, con
     if (act < ET_ACT_NONE || act > ET_ACT_GELU) return ET_ERR_INVALID_ARG;
     const int st = et::check_w4(in, out, group);
     if (st != ET_OK) return st;
-    if (T > 65535 * 16) return ET_ERR_SHAPE;
+    if (T > 65535 * 128) return ET_ERR_SHAPE;
     if (!et::aligned16(codes) || !et::aligned16(params) || !et::aligned16(X) || !et::aligned16(Y))
         return ET_ERR_ALIGNMENT;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool few = et::g_w4_small >= 0 ? et::g_w4_small != 0 : T <= et::W4_SMALL_T;
-    if (!few)
+    if (!et::w4_few_pay(T, in, out))
         return et::launch_linear_expand_w4(codes, reinterpret_cast<const __half*>(params), group,
                                            reinterpret_cast<const __half*>(bias),
                                            reinterpret_cast<const __half*>(X), reinterpret_cast<__half*>(Y), T, in,
@@ -440,9 +427,9 @@ int et_linear_w4_fwd(const uint8_t* codes, const et_half* params, int group, con
     a.T = T, a.in = in, a.out = out, a.act = act;
     a.nb = (in + 127) / 128;
     a.panels = out / 16;
-    if (group == 128) return et::launch_w4_tokens<1>(a, s);
-    if (group == 64) return et::launch_w4_tokens<2>(a, s);
-    return et::launch_w4_tokens<4>(a, s);
+    if (group == 128) return et::plan_w4<1>(a, s);
+    if (group == 64) return et::plan_w4<2>(a, s);
+    return et::plan_w4<4>(a, s);
 }
 
 }  // extern "C"

@@ -439,16 +439,16 @@ def _check_linear(et, cuda, T, inn, out, group, act=0, bias=True, seed=0, size=1
     x = (rng.normal(0, 1, (T, inn)) * size).astype(np.float16)
     b = rng.normal(0, 0.5, out).astype(np.float16) if bias else None
     if small is not None:
-        et.lib().et_debug_set_w4_small(small)
+        et.lib().et_debug_set_w4_few(small)
     try:
         y = et.linear_w4(_dev(x, cuda), q, None if b is None else _dev(b, cuda), act).cpu().numpy().astype(np.float64)
     finally:
         if small is not None:
-            et.lib().et_debug_set_w4_small(-1)
+            et.lib().et_debug_set_w4_few(-1)
     assert et.device_error() == 0
     lin = x.astype(np.float64) @ w64.T + (0 if b is None else b.astype(np.float64))
     want = lin if act == 0 else np.maximum(lin, 0) if act == 1 else _gelu(lin)
-    few = T <= 32 if small is None else small == 1
+    few = et.lib().et_debug_w4_few_pay(T, inn, out) if small is None else small == 1
     ax = np.abs(x.astype(np.float64))
     # fp32 sums: of c s x and m x apart, each in blocks of 128
     parts = ref.values(c, s, np.zeros_like(m))[:, :inn] + np.abs(ref.values(np.zeros_like(c), s, m)[:, :inn])

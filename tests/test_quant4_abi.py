@@ -124,7 +124,7 @@ def test_linear_w4_refuses(et):
 
     before = lib.et_launch_count()
     for bad, st in ((dict(codes=None), -1), (dict(params=None), -1), (dict(X=None), -1), (dict(Y=None), -1),
-                    (dict(T=0), -1), (dict(act=3), -1), (dict(group=48), -3), (dict(inn=120), -3), (dict(out=24), -3),
+                    (dict(T=0), -1), (dict(T=65535 * 128 + 1), -3), (dict(act=3), -1), (dict(group=48), -3), (dict(inn=120), -3), (dict(out=24), -3),
                     (dict(X=0x3008), -2), (dict(Y=0x4004), -2), (dict(codes=0x1008), -2), (dict(params=0x2004), -2)):
         assert fwd(**bad) == st, bad
     lib.et_w4_pack.argtypes = [P, I, I, I, P, P, P]
@@ -135,6 +135,15 @@ def test_linear_w4_refuses(et):
     assert lib.et_w4_densify(0x1000, 0x2000, 128, 64, 64, None, None) == -1
     assert lib.et_w4_densify(0x1000, 0x2000, 128, 60, 64, 0x3000, None) == -3
     assert lib.et_launch_count() == before
+
+
+def test_linear_w4_plan(et):
+    """Few tokens never expand the weights, many always do, and one side gives way to the other once."""
+    few = et.lib().et_debug_w4_few_pay
+    for inn, out in ((8192, 8192), (4096, 1024), (768, 2304), (1024, 4096), (512, 512), (16, 16), (8192, 28672)):
+        chosen = [few(t, inn, out) for t in (1, 8, 16, 32, 64, 128, 512, 4096)]
+        assert chosen[:2] == [1, 1] and chosen[-1] == 0, (inn, out, chosen)
+        assert chosen == sorted(chosen, reverse=True), (inn, out, chosen)
 
 
 def test_cached_layer_refuses(et):
