@@ -360,18 +360,21 @@ def _require(name: str, dtype, *tensors) -> None:
     """Tensors of a call: of one type, on the current device, with contiguous rows."""
     dev = _torch_c()._cuda_getDevice()
     for t in tensors:
-        if t is not None and (t.dtype is not dtype or t.get_device() != dev or (t.dim() and t.stride(-1) != 1)):
-            if t.dtype is not dtype:
-                raise EtError(f"{name}: a tensor is {t.dtype}, {dtype} is wanted")
-            if t.get_device() != dev:
-                raise EtError(f"{name}: a tensor is on {t.device}, the current device is cuda:{dev}")
-            if t.shape[-1] != 1:
-                raise EtError(f"{name}: the values of a row must be contiguous")
+        if t is None or (t.dtype is dtype and t.get_device() == dev and t.is_contiguous()):
+            continue
+        if t.dtype is not dtype:
+            raise EtError(f"{name}: a tensor is {t.dtype}, {dtype} is wanted")
+        if t.get_device() != dev:
+            raise EtError(f"{name}: a tensor is on {t.device}, the current device is cuda:{dev}")
+        if t.dim() and t.stride(-1) != 1 and t.shape[-1] != 1:
+            raise EtError(f"{name}: the values of a row must be contiguous")
 
 
-def _row_stride(t) -> int:
+def _row_stride(t, width: int) -> int:
     """Stride of a matrix's rows (a single row may report any)."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    if t.is_contiguous():
+        return width
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width)
 
 
 _F16 = _I32 = None  # torch's types, once torch is loaded
@@ -610,7 +613,7 @@ def _check_pages(name: str, cache: "KV4Cache", batch: int, table, *lengths) -> N
     if table.dim() != 2 or table.shape[0] != batch:
         raise EtError(f"{name}: a page table [{batch}, pages] is wanted")
     for n in lengths:
-        if n is not None and (n.dim() != 1 or n.shape[0] != batch):
+        if n is not None and (n.numel() != batch or not n.is_contiguous()):
             raise EtError(f"{name}: one length per sequence ({batch}) is wanted")
 
 
@@ -626,8 +629,8 @@ def kv4_write(cache: "KV4Cache", k, v, table, start, batch: int, seq: int, new_l
     _check_pages("kv4_write", cache, batch, table, start, new_len)
     _check_rows("kv4_write", "k", k, batch * seq, cache.k_width)
     _check_rows("kv4_write", "v", v, batch * seq, cache.v_width)
-    _call("et_kv4_write_fwd", cache._at, k.data_ptr(), v.data_ptr(), _row_stride(k), _row_stride(v), table.data_ptr(),
-          _row_stride(table), _a(start), _a(new_len), batch, seq, _raw_stream())
+    _call("et_kv4_write_fwd", cache._at, k.data_ptr(), v.data_ptr(), _row_stride(k, cache.k_width),
+          _row_stride(v, cache.v_width), table.data_ptr(), _row_stride(table, table.shape[1]), _a(start), _a(new_len), batch, seq, _raw_stream())
 
 
 def kv4_read(cache: "KV4Cache", table, batch: int, seq: int, start=None, length=None, out=None):
@@ -643,8 +646,8 @@ def kv4_read(cache: "KV4Cache", table, batch: int, seq: int, start=None, length=
         _require("kv4_read", f16, k, v)
         _check_rows("kv4_read", "k", k, rows, cache.k_width)
         _check_rows("kv4_read", "v", v, rows, cache.v_width)
-    _call("et_kv4_read_fwd", cache._at, k.data_ptr(), v.data_ptr(), _row_stride(k), _row_stride(v), table.data_ptr(),
-          _row_stride(table), _a(start), _a(length), batch, seq, _raw_stream())
+    _call("et_kv4_read_fwd", cache._at, k.data_ptr(), v.data_ptr(), _row_stride(k, cache.k_width),
+          _row_stride(v, cache.v_width), table.data_ptr(), _row_stride(table, table.shape[1]), _a(start), _a(length), batch, seq, _raw_stream())
     return k, v
 
 
@@ -670,7 +673,7 @@ def attention_kv4(cache: "KV4Cache", q, table, kv_len, batch: int, seq: int, nhe
     if mask is not None:
         if mask.dim() != 2 or mask.shape[0] < seq or mask.shape[1] < max_len:
             raise EtError(f"attention_kv4: a mask [{seq}, {max_len}] is wanted")
-        ldm = _row_stride(mask)
+        ldm = _row_stride(mask, mask.shape[1])
     n = 0
     if workspace is None:
         n = cache.workspace_bytes(batch, seq, nhead, max_len)
@@ -678,8 +681,9 @@ def attention_kv4(cache: "KV4Cache", q, table, kv_len, batch: int, seq: int, nhe
             workspace = q.new_empty((n + 1) // 2)
     else:
         n = workspace.numel() * workspace.element_size()
-    _call("et_attention_kv4_fwd", cache._at, q.data_ptr(), z.data_ptr(), table.data_ptr(), _row_stride(table),
-          kv_len.data_ptr(), _a(q_len), batch, seq, nhead, _row_stride(q), _row_stride(z), max_len, mask_kind, _a(mask),
+    _call("et_attention_kv4_fwd", cache._at, q.data_ptr(), z.data_ptr(), table.data_ptr(),
+          _row_stride(table, table.shape[1]), kv_len.data_ptr(), _a(q_len), batch, seq, nhead,
+          _row_stride(q, nhead * cache.dh_qk), _row_stride(z, nhead * cache.dh_v), max_len, mask_kind, _a(mask),
           ldm, cache.scale if scale is None else scale, _a(workspace), n, _raw_stream())
     return z
 
@@ -863,7 +867,7 @@ class EncoderLayer:
         if not x.is_contiguous() or not out.is_contiguous():
             raise EtError("forward_cached: contiguous x and out are wanted")
         _call("et_encoder_layer_cached_fwd", ctypes.addressof(self.desc), cache._at, _a(x), _a(out), batch, seq,
-              _a(table), _row_stride(table), _a(start), _a(kv_len), _a(new_len), max_len, _a(workspace),
+              _a(table), _row_stride(table, table.shape[1]), _a(start), _a(kv_len), _a(new_len), max_len, _a(workspace),
               workspace.numel() * workspace.element_size(), _raw_stream())
         return out
 
