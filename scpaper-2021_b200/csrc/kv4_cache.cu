@@ -7,7 +7,10 @@
 // eight consecutive tokens of a head: its rows lie together in the cache (ng = 2: 256 bytes of codes, 64 of
 // parameters), and a token's head is a whole line or more of the fp16 side anyway.
 //
-// What bounds it: HBM (2 + 0.625 bytes a value each way).
+// What bounds it.  Reading: HBM (4 x 8191 tokens, 8 heads of 128: 30.1 us, 5.8 TB/s).  Writing: instruction issue, 18 per
+// value and lane (8 x 2048 tokens, 16 heads of 64: about 28 us, 3.1 TB/s).  Registers are held down for more warps
+// (write + read back of those: 44.9 us; 46.3 where the compiler chose, 57.2 where it took what it liked); several
+// heads to a warp, the next one's values in flight, took 50.0.
 #include "kernels.h"
 #include "kv4.h"
 #include "quant4.cuh"
@@ -15,7 +18,7 @@
 namespace et {
 namespace {
 
-constexpr int KV_THREADS = 256;
+constexpr int KV_THREADS = 128;
 
 // x / d for 0 <= x < 2^31 by a multiplication
 struct FastDiv {
@@ -83,8 +86,11 @@ __device__ __forceinline__ void words_of_units(const uint32_t (&u)[NG], uint32_t
     }
 }
 
-template <int NG, bool WRITE>
-__global__ void __launch_bounds__(KV_THREADS) kv4_move_kernel(const Kv4Move a) {
+// FULL: both heads are 32 NG features wide.
+template <int NG, bool WRITE, bool FULL>
+__global__ void __launch_bounds__(KV_THREADS, NG <= 2 ? 12 : (NG == 3 ? 8 : 6)) kv4_move_kernel(const Kv4Move a) {
+    const int dh[2] = {FULL ? 32 * NG : a.c.dh[0], FULL ? 32 * NG : a.c.dh[1]};
+    auto inside = [&](int of, int first) { return FULL || first < dh[of]; };  // a feature of the head
     pdl_wait();
     pdl_launch_dependents();
     // unit: (eight tokens, head, token of the eight), four lanes each
@@ -101,12 +107,12 @@ __global__ void __launch_bounds__(KV_THREADS) kv4_move_kernel(const Kv4Move a) {
     __half* x[2];
 #pragma unroll
     for (int of = 0; of < 2; ++of) {
-        x[of] = a.x[of] + token * a.ld[of] + head * a.c.dh[of] + 8 * j;
+        x[of] = a.x[of] + token * a.ld[of] + head * dh[of] + 8 * j;
         if (WRITE)
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 v[of][g] = make_uint4(0, 0, 0, 0);
-                if (live && 32 * g + 8 * j < a.c.dh[of])
+                if (live && inside(of, 32 * g + 8 * j))
                     v[of][g] = __ldcg(reinterpret_cast<const uint4*>(x[of] + 32 * g));
             }
     }
@@ -139,7 +145,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv4_move_kernel(const Kv4Move a) {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const int of = k / NG, g = k % NG;
-            r[k] = k < 2 * NG && 32 * g + 8 * j < a.c.dh[of & 1] ? q4::range8(v[of & 1][g]) : q4::EMPTY_RANGE;
+            r[k] = k < 2 * NG && inside(of & 1, 32 * g + 8 * j) ? q4::range8(v[of & 1][g]) : q4::EMPTY_RANGE;
         }
 #pragma unroll
         for (int k = 0; k < N; k += 4) {
@@ -149,7 +155,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv4_move_kernel(const Kv4Move a) {
             const uint32_t hi = q4::range_join(one ? r[k + 3] : r[k + 2],
                                                __shfl_xor_sync(0xffffffffu, one ? r[k + 2] : r[k + 3], 1));
             const uint32_t mine = q4::range_join(two ? hi : lo, __shfl_xor_sync(0xffffffffu, two ? lo : hi, 2));
-            const uint32_t p = mine == q4::EMPTY_RANGE ? 0u : q4::params_of(mine);
+            const uint32_t p = (!FULL || k + 4 > 2 * NG) && mine == q4::EMPTY_RANGE ? 0u : q4::params_of(mine);
             const float i1 = q4::inverse_of(p);
 #pragma unroll
             for (int q = 0; q < 4; ++q)
@@ -169,7 +175,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv4_move_kernel(const Kv4Move a) {
             for (int g = 0; g < NG; ++g) {
                 const uint32_t c = of == 0 ? q4::codes8<true>(v[of][g], sm[of][g], inv[of][g])
                                            : q4::codes8<false>(v[of][g], sm[of][g], inv[of][g]);
-                w[g] = 32 * g + 8 * j < a.c.dh[of] ? c : 0u;
+                w[g] = inside(of, 32 * g + 8 * j) ? c : 0u;
                 if (g == j) mine = sm[of][g];
             }
             if (there) {
@@ -192,7 +198,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv4_move_kernel(const Kv4Move a) {
             }
 #pragma unroll
             for (int g = 0; g < NG; ++g)
-                if (32 * g + 8 * j < a.c.dh[of])
+                if (inside(of, 32 * g + 8 * j))
                     *reinterpret_cast<uint4*>(x[of] + 32 * g) =
                         of == 0 ? q4::values8<true>(w[g], sm[of][g]) : q4::values8<false>(w[g], sm[of][g]);
         }
@@ -221,9 +227,12 @@ int move(const et_kv4_t* cache, __half* K, __half* V, int ldk, int ldv, const in
     const int64_t blocks = (units + KV_THREADS / 32 - 1) / (KV_THREADS / 32);
     a.err_word = device_error_word();
     if (!a.err_word) return ET_ERR_NO_DEVICE;
-    void (*const kernels[4])(const Kv4Move) = {kv4_move_kernel<1, WRITE>, kv4_move_kernel<2, WRITE>,
-                                               kv4_move_kernel<3, WRITE>, kv4_move_kernel<4, WRITE>};
-    return launch_kernel(kernels[a.c.ng - 1], dim3(static_cast<unsigned>(blocks)), dim3(KV_THREADS), 0, stream, a) ==
+    void (*const kernels[8])(const Kv4Move) = {
+        kv4_move_kernel<1, WRITE, false>, kv4_move_kernel<2, WRITE, false>, kv4_move_kernel<3, WRITE, false>,
+        kv4_move_kernel<4, WRITE, false>, kv4_move_kernel<1, WRITE, true>,  kv4_move_kernel<2, WRITE, true>,
+        kv4_move_kernel<3, WRITE, true>,  kv4_move_kernel<4, WRITE, true>};
+    const bool full = a.c.dh[0] == 32 * a.c.ng && a.c.dh[1] == 32 * a.c.ng;
+    return launch_kernel(kernels[a.c.ng - 1 + (full ? 4 : 0)], dim3(static_cast<unsigned>(blocks)), dim3(KV_THREADS), 0, stream, a) ==
                    cudaSuccess
                ? ET_OK
                : ET_ERR_CUDA;
