@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
     constexpr int D = 32 * NG, STAGES = S::STAGES, TILE = S::TILE;
     constexpr int HALVES = TILE / 16;  // 16 tokens lie in one page
     extern __shared__ __align__(128) uint8_t smem[];
-    const int warp = uniform_warp_id(), lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int i = lane >> 2, j = lane & 3;
     const int tau = (i >> 1) + 4 * (i & 1);
     uint8_t* ring = smem + warp * S::WARP;
