@@ -36,6 +36,7 @@ namespace {
 constexpr int WARPS = 4;
 constexpr int THREADS = 32 * WARPS;
 constexpr int MAX_SPLITS = 64;
+constexpr int JOIN_AHEAD = 16;  // partial results that the second kernel has in flight
 constexpr int MIN_CHUNK = 256;  // tokens of a split at least: two tiles per warp
 constexpr int MAX_CLUSTER = 8;  // splits that join through distributed shared memory
 constexpr float LOG2E = 1.4426950408889634f;
@@ -51,8 +52,9 @@ struct AttArgs {
     float* part;   // [splits][rows][32 ng] sums, then [splits][rows][2] (reference, sum of p)
     float* part_ml;
     int table_ld, batch, seq, nhead, ratio, ldq, ldz, ldm, max_len, mask_kind;
-    int rows, tiles;  // query rows per (sequence, key/value head), row tiles
-    int splits;
+    int tiles;        // of query rows per (sequence, key/value head)
+    int splits, per;  // blocks along the sequence, tokens of each
+    FastDiv by_ratio;
     float scale_log2;
     int* err_word;
 };
@@ -197,48 +199,63 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
     const int split = blockIdx.x;
     const int rt = blockIdx.y % a.tiles, kvh = blockIdx.y / a.tiles;
     const int b = blockIdx.z;
+    const int row0 = rt * 8 * NT;  // row r is query token r / ratio, head kvh * ratio + r % ratio
+
+    // ---- everything that waits for nothing is asked for at once: lengths, queries, page numbers
     int len = __ldcg(a.kv_len + b);
+    int nq = a.q_len ? __ldcg(a.q_len + b) : a.seq;
+    uint32_t qf[NG][NT][4];  // row 8 t + i: features 32 g + 8 j .. + 8
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int r = row0 + 8 * t + i, qi = a.by_ratio.div(r), head = kvh * a.ratio + r - qi * a.ratio;
+        const __half* q = a.Q + (static_cast<int64_t>(b) * a.seq + qi) * a.ldq + head * a.c.dh[0] + 8 * j;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (qi < a.seq && 32 * g + 8 * j < a.c.dh[0]) v = __ldcg(reinterpret_cast<const uint4*>(q + 32 * g));
+            qf[g][t][0] = v.x, qf[g][t][1] = v.y, qf[g][t][2] = v.z, qf[g][t][3] = v.w;
+        }
+    }
+    // Page numbers, of 16 tokens to a lane, BATCH tiles at a time; the warp's tiles are warp, warp + 4, ... of the
+    // block's chunk.  What the table holds past the sequence's end is read, but neither followed nor reported.
+    constexpr int BATCH = 32 / HALVES;
+    const int first = split * a.per;
+    const int* table = a.table + static_cast<int64_t>(b) * a.table_ld;
+    auto position = [&](int n) { return first + ((n + lane / HALVES) * WARPS + warp) * TILE + lane % HALVES * 16; };
+    auto entry = [&](int n) {
+        const int pos = position(n), e = pos >> a.c.page_shift;
+        return pos < a.max_len && e < a.table_ld ? __ldcg(table + e) : -1;
+    };
+    int raw = entry(0), raw_next = entry(BATCH);
+
     if (len > a.max_len) {
         if (threadIdx.x == 0) atomicCAS(a.err_word, 0, DEV_BAD_PAGE);
         len = a.max_len;
     }
     len = len < 0 ? 0 : len;
-    int nq = a.q_len ? __ldcg(a.q_len + b) : a.seq;
     nq = nq < 0 ? 0 : (nq > a.seq ? a.seq : nq);
-
-    // ---- rows: row r of the tile is query token r / ratio, head kvh * ratio + r % ratio
-    const int row0 = rt * 8 * NT;
     if (row0 >= nq * a.ratio) return;  // (rows are ordered by query token)
     int most, least;  // the largest and smallest number of tokens that a row sees: the last and first row's
     {
         const int last = (row0 + 8 * NT < nq * a.ratio ? row0 + 8 * NT : nq * a.ratio) - 1;
         if (a.mask_kind == ET_MASK_CAUSAL) {
-            least = len - nq + row0 / a.ratio + 1;
-            most = len - nq + last / a.ratio + 1;
+            least = len - nq + static_cast<int>(a.by_ratio.div(row0)) + 1;
+            most = len - nq + static_cast<int>(a.by_ratio.div(last)) + 1;
         } else {
             least = most = len;
         }
         most = most < 0 ? 0 : most;
     }
-    // this block's chunk of the sequence, and the warp's tiles in it: warp, warp + 4, ...
-    const int per = ((most + a.splits - 1) / a.splits + TILE - 1) / TILE * TILE;
-    const int64_t first64 = static_cast<int64_t>(split) * per;
-    const int first = first64 < most ? static_cast<int>(first64) : most;
-    const int end = first + per < most ? first + per : most;
-    const int ntile = (end - first + TILE - 1) / TILE;
+    const int end = first + a.per < most ? first + a.per : most;  // of this block's chunk
+    const int ntile = end > first ? (end - first + TILE - 1) / TILE : 0;
     const int mine = ntile > warp ? (ntile - warp + WARPS - 1) / WARPS : 0;
-
-    // ---- page numbers, of 16 tokens to a lane: BATCH tiles at a time
-    constexpr int BATCH = 32 / HALVES;
-    const int* table = a.table + static_cast<int64_t>(b) * a.table_ld;
-    auto page_of = [&](int n) {  // of the lane's share of the tiles from tile n on; -1: nothing to read
-        const int pos = first + ((n + lane / HALVES) * WARPS + warp) * TILE + lane % HALVES * 16;
-        if (pos >= end || n + lane / HALVES >= mine) return -1;
-        const int id = kv4_page(a.c, table, a.table_ld, pos);
-        if (id < 0) atomicCAS(a.err_word, 0, DEV_BAD_PAGE);
-        return id;
+    auto checked = [&](int n, int id) {  // page of the lane's 16 tokens, or -1: nothing to read
+        if (position(n) >= end || n + lane / HALVES >= mine) return -1;
+        if (id >= 0 && id < a.c.num_pages) return id;
+        atomicCAS(a.err_word, 0, DEV_BAD_PAGE);
+        return -1;
     };
-    int pages = page_of(0), pages_next = page_of(BATCH);
+    int pages = checked(0, raw), pages_next = checked(BATCH, raw_next);
     // Copies tile n of this warp (called with n = 0, 1, 2, ... in order), zeros where nothing is to be read: per 16
     // tokens 16 NG pieces of 16 bytes of either codes and 4 NG of either parameters (K's by lanes 0 .., V's by
     // lanes 16 ..).
@@ -250,7 +267,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
         if (n < mine) {
             if (n != 0 && n % BATCH == 0) {
                 pages = pages_next;
-                pages_next = page_of(n + BATCH);
+                pages_next = checked(n + BATCH, entry(n + BATCH));
             }
             const uint32_t st = ring32 + (n % STAGES) * S::STAGE;
             const int pos = first + (n * WARPS + warp) * TILE;
@@ -277,24 +294,16 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
 
     // ---- the rows' queries, scaled by a power of two of their own to at most 2^11: lossless, and room for the
     // factor 16 that makes up for the nibbles which K's codes are multiplied at (4 bits up, every second pair)
-    int limit[NT][2];        // tokens that rows 8 t + 2 j, 8 t + 2 j + 1 see
-    uint32_t qf[NG][NT][4];  // row 8 t + i: features 32 g + 8 j .. + 8, in pairs: times 16, 1, 16, 1
-    uint64_t qs[NG][NT];     // rows 8 t + 2 j, + 1: sums over the group, in the units of the first product
-    float unit[NT][2];       // those units times scale and log2(e)
+    int limit[NT][2];     // tokens that rows 8 t + 2 j, 8 t + 2 j + 1 see
+    uint64_t qs[NG][NT];  // rows 8 t + 2 j, + 1: sums over the group, in the units of the first product
+    float unit[NT][2];    // those units times scale and log2(e)
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const int r = row0 + 8 * t + i;
-        const int qi = r / a.ratio, head = kvh * a.ratio + r % a.ratio;
-        const __half* q = a.Q + (static_cast<int64_t>(b) * a.seq + qi) * a.ldq + head * a.c.dh[0] + 8 * j;
         uint32_t big = 0;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (qi < nq && 32 * g + 8 * j < a.c.dh[0]) v = __ldcg(reinterpret_cast<const uint4*>(q + 32 * g));
-            qf[g][t][0] = v.x, qf[g][t][1] = v.y, qf[g][t][2] = v.z, qf[g][t][3] = v.w;
+        for (int g = 0; g < NG; ++g)
 #pragma unroll
             for (int k = 0; k < 4; ++k) big = max(big, max(qf[g][t][k] & 0x7fffu, (qf[g][t][k] >> 16) & 0x7fffu));
-        }
         big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
         big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
         // 2^k, k = 10 - exponent of the largest (0 for rows of zeros and rows that are not finite)
@@ -321,7 +330,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             unit[t][h] = __shfl_sync(0xffffffffu, down, 8 * j + 4 * h);
-            const int qr = (row0 + 8 * t + 2 * j + h) / a.ratio;
+            const int qr = a.by_ratio.div(row0 + 8 * t + 2 * j + h);
             // (rows that are not there compute on zero queries and are never stored)
             limit[t][h] = qr >= nq ? (a.mask_kind == ET_MASK_ADDITIVE ? 0 : INT32_MAX)
                                    : (a.mask_kind == ET_MASK_CAUSAL ? len - nq + qr + 1 : len);
@@ -430,7 +439,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
                 for (int h = 0; h < 2; ++h) {
                     const float per_unit = LOG2E / unit[t][h];
                     const __half* mrow =
-                        a.mask + static_cast<int64_t>((row0 + 8 * t + 2 * j + h) / a.ratio) * a.ldm;
+                        a.mask + static_cast<int64_t>(a.by_ratio.div(row0 + 8 * t + 2 * j + h)) * a.ldm;
 #pragma unroll
                     for (int k = 0; k < 2 * HALVES; ++k) {
                         const int tok = tok0 + 8 * k + tau;
@@ -621,7 +630,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
     const bool clustered = a.splits > 1 && a.splits <= MAX_CLUSTER;
     for (int u = threadIdx.x; u < ROWS * (D / 8); u += THREADS) {
         const int r = u / (D / 8), d = (u - r * (D / 8)) * 8;
-        const int rr = row0 + r, qi = rr / a.ratio, head = kvh * a.ratio + rr % a.ratio;
+        const int rr = row0 + r, qi = a.by_ratio.div(rr), head = kvh * a.ratio + rr - qi * a.ratio;
         if (qi >= nq) continue;
         float o[8], top_all, sum;
         join_partials<WARPS>(WARPS, o, top_all, sum, [&](int w) { return xml + 2 * (w * ROWS + r); },
@@ -650,7 +659,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
     const uint32_t x32 = smem_u32(mine_x), ml32 = smem_u32(mine_ml);
     for (int u = threadIdx.x * a.splits + split; u < ROWS * (D / 8); u += a.splits * THREADS) {
         const int r = u / (D / 8), d = (u - r * (D / 8)) * 8;
-        const int rr = row0 + r, qi = rr / a.ratio, head = kvh * a.ratio + rr % a.ratio;
+        const int rr = row0 + r, qi = a.by_ratio.div(rr), head = kvh * a.ratio + rr - qi * a.ratio;
         if (qi >= nq || d >= a.c.dh[1]) continue;
         float o[8], top_all, sum;
         join_partials<MAX_CLUSTER>(a.splits, o, top_all, sum,
@@ -687,14 +696,23 @@ __global__ void __launch_bounds__(128) attention_kv4_join_kernel(const AttArgs a
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < a.splits; ++s) {
-        const float f = __shfl_sync(0xffffffffu, s < 32 ? t0 : t1, s & 31);
-        if (f != 0.f && 4 * lane < D) {  // (f = 0 also where the split saw nothing; NaN passes)
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part + (s * all + at) * D) + lane);
-            o.x = fmaf(v.x, f, o.x);
-            o.y = fmaf(v.y, f, o.y);
-            o.z = fmaf(v.z, f, o.z);
-            o.w = fmaf(v.w, f, o.w);
+    for (int s0 = 0; s0 < a.splits; s0 += JOIN_AHEAD) {
+        float4 v[JOIN_AHEAD];
+#pragma unroll
+        for (int k = 0; k < JOIN_AHEAD; ++k) {
+            const int s = s0 + k < a.splits ? s0 + k : a.splits - 1;  // (the last again: its factor is 0 below)
+            v[k] = __ldcg(reinterpret_cast<const float4*>(a.part + (s * all + at) * D) + (4 * lane < D ? lane : 0));
+        }
+#pragma unroll
+        for (int k = 0; k < JOIN_AHEAD; ++k) {
+            const int s = s0 + k;
+            const float f = __shfl_sync(0xffffffffu, s < 32 ? t0 : t1, s & 31);
+            if (f != 0.f && s < a.splits) {  // (0 also where the split saw nothing; NaN passes)
+                o.x = fmaf(v[k].x, f, o.x);
+                o.y = fmaf(v[k].y, f, o.y);
+                o.z = fmaf(v[k].z, f, o.z);
+                o.w = fmaf(v[k].w, f, o.w);
+            }
         }
     }
     if (4 * lane < a.c.dh[1]) {
@@ -813,9 +831,10 @@ int et_attention_kv4_fwd(const et_kv4_t* cache, const et_half* Q, et_half* Z, co
     a.batch = batch, a.seq = seq, a.nhead = nhead, a.ratio = nhead / a.c.nkv;
     a.ldq = ldq, a.ldz = ldz, a.ldm = ldm, a.max_len = max_len;
     a.mask_kind = mask_kind;
-    a.rows = seq * a.ratio;
+    a.by_ratio = et::FastDiv(static_cast<uint32_t>(a.ratio));
     a.tiles = p.tiles;
     a.splits = p.splits;
+    a.per = ((max_len + p.splits - 1) / p.splits + 31) / 32 * 32;  // whole tiles
     a.scale_log2 = scale * et::LOG2E;
     a.err_word = et::device_error_word();
     if (!a.err_word) return ET_ERR_NO_DEVICE;

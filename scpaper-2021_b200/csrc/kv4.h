@@ -3,6 +3,12 @@
 
 #include "common.cuh"
 
+#if defined(__CUDACC__)
+#define KV4_HD __host__ __device__ __forceinline__
+#else
+#define KV4_HD inline
+#endif
+
 namespace et {
 
 struct Kv4View {
@@ -37,6 +43,20 @@ inline int kv4_view(const et_kv4_t* c, Kv4View& v, bool pointers) {
     v.ng = ((c->dh_qk > c->dh_v ? c->dh_qk : c->dh_v) + 31) / 32;
     return ET_OK;
 }
+
+// x / d for 0 <= x < 2^31 by a multiplication
+struct FastDiv {
+    uint32_t mul, shift, d;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t d_) : d(d_) {
+        shift = 0;
+        while ((1u << shift) < d && shift < 31) ++shift;
+        mul = static_cast<uint32_t>(((1ull << (31 + shift)) + d - 1) / d);
+    }
+    KV4_HD uint32_t div(uint32_t x) const {
+        return static_cast<uint32_t>((static_cast<uint64_t>(x) * mul) >> (31 + shift));
+    }
+};
 
 // Sizes that the attention over the cache takes (its grid, and 32-bit counts of rows and positions).
 inline int kv4_check_attention(const Kv4View& v, int batch, int seq, int nhead, int max_len) {

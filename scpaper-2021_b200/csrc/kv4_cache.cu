@@ -20,20 +20,6 @@ namespace {
 
 constexpr int KV_THREADS = 128;
 
-// x / d for 0 <= x < 2^31 by a multiplication
-struct FastDiv {
-    uint32_t mul, shift, d;
-    FastDiv() = default;
-    explicit FastDiv(uint32_t d_) : d(d_) {
-        shift = 0;
-        while ((1u << shift) < d && shift < 31) ++shift;
-        mul = static_cast<uint32_t>(((1ull << (31 + shift)) + d - 1) / d);
-    }
-    __host__ __device__ __forceinline__ uint32_t div(uint32_t x) const {
-        return static_cast<uint32_t>((static_cast<uint64_t>(x) * mul) >> (31 + shift));
-    }
-};
-
 struct Kv4Move {
     Kv4View c;
     __half* x[2];  // fp16 K and V
