@@ -671,42 +671,43 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
     cluster_sync_all();  // (no block leaves while another reads its shared memory)
 }
 
-// Joins the splits' partial results: a warp per (row, head), four features per lane.
-__global__ void __launch_bounds__(128) attention_kv4_join_kernel(const AttArgs a) {
+// Joins the splits' partial results: a warp per (row, head), four features per lane.  What it takes is one trip to
+// memory and the launch; the sums are asked for before their factors are known.
+__global__ void __launch_bounds__(64) attention_kv4_join_kernel(const AttArgs a) {
     pdl_wait();
     pdl_launch_dependents();
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    const int64_t all = static_cast<int64_t>(a.batch) * a.seq * a.nhead;
+    const int all = a.batch * a.seq * a.nhead, at = blockIdx.x * 2 + (threadIdx.x >> 5);
     if (at >= all) return;
-    const int64_t row = at / a.nhead;
-    const int head = static_cast<int>(at - row * a.nhead), b = static_cast<int>(row / a.seq);
-    const int qi = static_cast<int>(row - static_cast<int64_t>(b) * a.seq);
-    if (a.q_len && qi >= __ldcg(a.q_len + b)) return;
+    const int row = at / a.nhead, head = at - row * a.nhead, b = row / a.seq;
+    if (a.q_len && row - b * a.seq >= __ldcg(a.q_len + b)) return;
     const int lane = threadIdx.x & 31, D = 32 * a.c.ng;
-    // splits <= 64: two references per lane
-    float t0 = lane < a.splits ? __ldcg(a.part_ml + 2 * (lane * all + at)) : -INFINITY;
-    float t1 = lane + 32 < a.splits ? __ldcg(a.part_ml + 2 * ((lane + 32) * all + at)) : -INFINITY;
-    float top = fmaxf(t0, t1);
+    const float4* part = reinterpret_cast<const float4*>(a.part + static_cast<int64_t>(at) * D) + (4 * lane < D ? lane : 0);
+    const int64_t next = static_cast<int64_t>(all) * D / 4;  // from a split to the next
+    auto load = [&](float4(&v)[JOIN_AHEAD], int s0) {
+#pragma unroll
+        for (int k = 0; k < JOIN_AHEAD; ++k)  // (past the last split that one again: its factor is 0 below)
+            v[k] = __ldcg(part + (s0 + k < a.splits ? s0 + k : a.splits - 1) * next);
+    };
+    float4 v[JOIN_AHEAD];
+    load(v, 0);
+    // splits <= 64: two of (reference, sum of p) per lane
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + at;
+    float2 m0 = make_float2(-INFINITY, 0.f), m1 = m0;
+    if (lane < a.splits) m0 = __ldcg(ml + static_cast<int64_t>(lane) * all);
+    if (lane + 32 < a.splits) m1 = __ldcg(ml + static_cast<int64_t>(lane + 32) * all);
+    float top = fmaxf(m0.x, m1.x);
 #pragma unroll
     for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    t0 = t0 == -INFINITY ? 0.f : exp2f(t0 - top);
-    t1 = t1 == -INFINITY ? 0.f : exp2f(t1 - top);
-    float sum = (lane < a.splits ? __ldcg(a.part_ml + 2 * (lane * all + at) + 1) * t0 : 0.f) +
-                (lane + 32 < a.splits ? __ldcg(a.part_ml + 2 * ((lane + 32) * all + at) + 1) * t1 : 0.f);
+    const float f0 = m0.x == -INFINITY ? 0.f : exp2f(m0.x - top), f1 = m1.x == -INFINITY ? 0.f : exp2f(m1.x - top);
+    float sum = m0.y * f0 + m1.y * f1;
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s0 = 0; s0 < a.splits; s0 += JOIN_AHEAD) {
-        float4 v[JOIN_AHEAD];
-#pragma unroll
-        for (int k = 0; k < JOIN_AHEAD; ++k) {
-            const int s = s0 + k < a.splits ? s0 + k : a.splits - 1;  // (the last again: its factor is 0 below)
-            v[k] = __ldcg(reinterpret_cast<const float4*>(a.part + (s * all + at) * D) + (4 * lane < D ? lane : 0));
-        }
+    for (int s0 = 0;;) {
 #pragma unroll
         for (int k = 0; k < JOIN_AHEAD; ++k) {
             const int s = s0 + k;
-            const float f = __shfl_sync(0xffffffffu, s < 32 ? t0 : t1, s & 31);
+            const float f = __shfl_sync(0xffffffffu, s < 32 ? f0 : f1, s & 31);
             if (f != 0.f && s < a.splits) {  // (0 also where the split saw nothing; NaN passes)
                 o.x = fmaf(v[k].x, f, o.x);
                 o.y = fmaf(v[k].y, f, o.y);
@@ -714,13 +715,15 @@ __global__ void __launch_bounds__(128) attention_kv4_join_kernel(const AttArgs a
                 o.w = fmaf(v[k].w, f, o.w);
             }
         }
+        if ((s0 += JOIN_AHEAD) >= a.splits) break;
+        load(v, s0);
     }
     if (4 * lane < a.c.dh[1]) {
         const float inv = top == -INFINITY ? 0.f : 1.f / sum;
         uint2 z;
         z.x = pack_half2(o.x * inv, o.y * inv);
         z.y = pack_half2(o.z * inv, o.w * inv);
-        *reinterpret_cast<uint2*>(a.Z + row * a.ldz + head * a.c.dh[1] + 4 * lane) = z;
+        *reinterpret_cast<uint2*>(a.Z + static_cast<int64_t>(row) * a.ldz + head * a.c.dh[1] + 4 * lane) = z;
     }
 }
 
@@ -851,7 +854,7 @@ int et_attention_kv4_fwd(const et_kv4_t* cache, const et_half* Q, et_half* Z, co
     }
     if (st != ET_OK || p.splits <= et::MAX_CLUSTER) return st;
     const int64_t all = static_cast<int64_t>(batch) * seq * nhead;
-    return et::launch_kernel(et::attention_kv4_join_kernel, dim3(static_cast<unsigned>((all + 3) / 4)), dim3(128), 0, s,
+    return et::launch_kernel(et::attention_kv4_join_kernel, dim3(static_cast<unsigned>((all + 1) / 2)), dim3(64), 0, s,
                              a) == cudaSuccess
                ? ET_OK
                : ET_ERR_CUDA;
