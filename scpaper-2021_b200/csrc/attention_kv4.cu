@@ -16,7 +16,7 @@
 // tokens) and a chunk of the sequence; its four warps take 32-token tiles in turn, each with a ring of asynchronous
 // copies of its own (page contents land in shared memory as they are; no thread waits for another warp in the
 // loop).  With few rows the sequence is split over the blocks of a cluster, which join their partial results
-// through distributed shared memory, or (more than 8) over blocks that leave them to a second kernel.
+// through distributed shared memory, or (more than 4) over blocks that leave them to a second kernel.
 //
 // Layout.  Both products have the cache as their 16-row operand and eight query rows as their 8-column one: a few
 // rows then waste little of the tensor core and of the registers (with the rows on the 16 side, half
@@ -38,7 +38,7 @@ constexpr int THREADS = 32 * WARPS;
 constexpr int MAX_SPLITS = 64;
 constexpr int JOIN_AHEAD = 16;  // partial results that the second kernel has in flight
 constexpr int MIN_CHUNK = 256;  // tokens of a split at least: two tiles per warp
-constexpr int MAX_CLUSTER = 8;  // splits that join through distributed shared memory
+constexpr int MAX_CLUSTER = 4;  // splits that join through distributed shared memory
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct AttArgs {
