@@ -235,7 +235,7 @@ int et_1x16_densify(const int32_t* tile_idx, const int32_t* row_idx, const et_ha
  *   et_linear_w4_fwd  the forward pass.  Few tokens: codes and fp16 activations are multiplied as they are,
  *     scales applied to fp32 sums (one pass over the 4-bit weights, no rounding of a weight); many tokens:
  *     the weights are expanded to fp16 operand tiles in shared memory in front of the tcgen05 product.
- *     An activation that is not finite leaves every output of its token without a finite value.
+ *     An activation that is not finite leaves no sum of its token finite (RELU then makes NaN 0).
  * codes, params, X, Y 16-byte aligned (bias: 2); in and out multiples of 16.  Like every weight, codes and
  * params must be complete (stream synchronised) before the first Linear call that uses them.  Stands beside
  * the weight formats of mat_type/; the reference has no quantised one. */
@@ -455,8 +455,10 @@ int et_kv4_read_fwd(const et_kv4_t* cache, et_half* K, et_half* V, int ldk, int 
  * A query that sees nothing (kv_len 0, or every score -inf) yields zeros.  What stands in a masked
  * place, NaN included, does not reach the output.
  * max_len: the largest kv_len (at most table_ld * page); longer sequences are cut there and
- * reported (601).  Q.K is exact up to fp32 sums (codes and fp16 queries are multiplied as they
- * are), probabilities enter the second product with 22 bits.
+ * reported (601).  scale: 2^-64 .. 2^64.  Q.K is exact up to fp32 sums (codes and fp16 queries are
+ * multiplied as they are); a probability times its group's scale enters the second product with 22
+ * bits, or to 2^-25 of the row's largest such product (groups of a head whose ranges lie 2^10 and
+ * more apart: the small ones are as precise as the large ones allow).
  * The long axis is split over thread blocks when there are few rows; their fp32 partial results
  * go to the workspace (et_attention_kv4_workspace_bytes; 0: none needed), which calls that may
  * overlap on the GPU must not share.  Nothing of it has to be set or kept.  */

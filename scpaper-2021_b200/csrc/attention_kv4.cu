@@ -9,8 +9,9 @@
 // with p s split into two fp16 numbers (22 bits) and one product for each.  (Codes less 8: sums of codes of one
 // sign grow with the sequence while the output shrinks, and the tensor core cuts its fp32 sums: at 32768 tokens
 // that cost half of the result's own rounding again, 3.2e-4 for 2.1e-4.)  The softmax is online; its reference is
-// the running maximum of the scaled scores plus the exponent of the running largest s, so that p s < 1 whatever
-// the magnitude of V.
+// a recent maximum, over the tokens that the row sees, of the scaled score plus the exponent of the token's largest s,
+// and moves when one passes it by 6: p s < 2^6 whatever the magnitude of V, and what is hidden from a row, or
+// too unlikely to count, costs it no precision.
 //
 // A thread block owns up to 16 query rows that share a key/value head (the heads of a group times the query
 // tokens) and a chunk of the sequence; its four warps take 32-token tiles in turn, each with a ring of asynchronous
@@ -102,7 +103,7 @@ __device__ __forceinline__ void lds_units(const uint8_t* p, uint32_t (&u)[(NG + 
 
 template <int NG, int NT>
 struct Shape {
-    static constexpr int TILE = 32;  // tokens of a warp's tile
+    static constexpr int TILE = 32;  // tokens of a warp's tile: one to a lane for the parameters
     static constexpr int STAGES = NG * TILE >= 128 ? 2 : 3;
     static constexpr int CODES = TILE * 16 * NG, PARAMS = TILE * 4 * NG;
     static constexpr int STAGE = 2 * (CODES + PARAMS);  // K codes, V codes, K params, V params
@@ -339,8 +340,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
 
     float acc[NG][2][NT][4];  // [group][u]: features f = 2 u (elements 0, 1) and, times 16, 2 u + 1 (2, 3)
     uint64_t pm[NG][NT];      // sums of p (m + 8 s), two rows
-    float l[NT][2], top[NT][2];  // sum of p, and the reference less e: -inf until the row sees a key
-    float e = -14.f;             // exponent: every s so far is < 2^e
+    float l[NT][2], top[NT][2];  // sum of p, and the reference: -inf until the row sees a key
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -361,39 +361,38 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
         const uint8_t* st = ring + (n % STAGES) * S::STAGE;
         const int tok0 = first + (n * WARPS + warp) * TILE;
 
-        // ---- K's (s, m) to fp32; V's largest s, and whether all of V's are finite
-        constexpr int TL = TILE / 32;  // tokens of a lane: lane, lane + 32
-        uint32_t vp[TL][NG], odd_bits = 0, s_top = 0;
-#pragma unroll
-        for (int q = 0; q < TL; ++q) {
-            const int tok = lane + 32 * q;
+        // ---- the lane's token: K's (s, m) to fp32; V's largest s, and whether all of V's are finite
+        uint32_t vp[NG], odd_bits = 0, s_top = 0;
+        {
             uint32_t kp[NG];
-            lds_words<NG>(st + 2 * S::CODES + tok * 4 * NG, kp);
-            lds_words<NG>(st + 2 * S::CODES + S::PARAMS + tok * 4 * NG, vp[q]);
-            if (tok0 + tok >= end) {  // not of this sequence, or this block's: counts as zeros
+            lds_words<NG>(st + 2 * S::CODES + lane * 4 * NG, kp);
+            lds_words<NG>(st + 2 * S::CODES + S::PARAMS + lane * 4 * NG, vp);
+            if (tok0 + lane >= end) {  // not of this sequence, or this block's: counts as zeros
 #pragma unroll
-                for (int g = 0; g < NG; ++g) kp[g] = vp[q][g] = 0u;
+                for (int g = 0; g < NG; ++g) kp[g] = vp[g] = 0u;
             }
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&kp[g]));
-                wide[tok * S::WIDE_LD + g] = make_float4(x.x, x.x, x.y, x.y);
-                odd_bits |= (vp[q][g] & 0x7c007c00u) + 0x04000400u;  // (an exponent of all ones carries)
-                s_top = max(s_top, vp[q][g] & 0x7fffu);
+                wide[lane * S::WIDE_LD + g] = make_float4(x.x, x.x, x.y, x.y);
+                odd_bits |= (vp[g] & 0x7c007c00u) + 0x04000400u;  // (an exponent of all ones carries)
+                s_top = max(s_top, vp[g] & 0x7fffu);
             }
         }
         const bool odd = __any_sync(0xffffffffu, (odd_bits & 0x80008000u) != 0);
         if (odd) {
             s_top = 0;
 #pragma unroll
-            for (int k = 0; k < TL * NG; ++k) {
-                uint32_t& w = vp[k / NG][k % NG];
-                if (!q4::finite16(w) || !q4::finite16(w >> 16)) w = 0u;
-                s_top = max(s_top, w & 0x7fffu);
+            for (int g = 0; g < NG; ++g) {
+                if (!q4::finite16(vp[g]) || !q4::finite16(vp[g] >> 16)) vp[g] = 0u;
+                s_top = max(s_top, vp[g] & 0x7fffu);
             }
         }
-        s_top = __reduce_max_sync(0xffffffffu, s_top);
-        const float e_new = fmaxf(e, static_cast<float>(static_cast<int>(s_top >> 10) - 14));
+        // every s of the token is < 2^e; e of tokens tau, tau + 8, ...
+        const float e_mine = static_cast<float>(static_cast<int>(s_top >> 10) - 14);
+        float e[2 * HALVES];
+#pragma unroll
+        for (int k = 0; k < 2 * HALVES; ++k) e[k] = __shfl_sync(0xffffffffu, e_mine, 8 * k + tau);
         __syncwarp();
 
         // ---- scores, in the row's units: [16-token block][token tau, tau + 8][row 2 j, 2 j + 1]
@@ -453,18 +452,18 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
                 }
         }
 
-        // ---- online softmax.  The reference moves only when a score passes it by 2^6 (or a larger s arrives): the
-        // lanes then need not agree on the tile's maximum, and p s < 2^6 is as good to fp16.
+        // ---- online softmax.  The reference moves only when a score plus e passes it by 6: the lanes then need not agree
+        // on the tile's maximum, and p s < 2^6 is as good to fp16.
         float mx[NT][2];
-        bool move = e_new > e;
+        bool move = false;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                mx[t][h] = x[0][t][0][h];
+                mx[t][h] = fmaf(x[0][t][0][h], unit[t][h], e[0]);
 #pragma unroll
-                for (int k = 1; k < 2 * HALVES; ++k) mx[t][h] = fmaxf(mx[t][h], x[k >> 1][t][k & 1][h]);
-                mx[t][h] *= unit[t][h];
+                for (int k = 1; k < 2 * HALVES; ++k)
+                    mx[t][h] = fmaxf(mx[t][h], fmaf(x[k >> 1][t][k & 1][h], unit[t][h], e[k]));
                 move = move || mx[t][h] > top[t][h] + 6.f;
             }
         if (__any_sync(0xffffffffu, move)) {
@@ -478,7 +477,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
                     m = fmaxf(m, top[t][h]);
                     // (a row that has seen nothing keeps sums of zero)
-                    shrink[h] = top[t][h] == -INFINITY ? 1.f : exp2f(top[t][h] - m + e - e_new);
+                    shrink[h] = top[t][h] == -INFINITY ? 1.f : exp2f(top[t][h] - m);
                     top[t][h] = m;
                     l[t][h] *= shrink[h];
                 }
@@ -489,13 +488,12 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
                     for (int k = 0; k < 8; ++k) acc[g][k >> 2][t][k & 3] *= shrink[k & 1];
                 }
             }
-            e = e_new;
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float ref = (top[t][h] == -INFINITY ? 0.f : top[t][h]) + e;
+                const float ref = top[t][h] == -INFINITY ? 0.f : top[t][h];
 #pragma unroll
                 for (int k = 0; k < 2 * HALVES; ++k) {
                     float& v = x[k >> 1][t][k & 1][h];
@@ -534,10 +532,10 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
         // ---- V's (s, m + 8 s) to fp32, in K's place
         __syncwarp();
 #pragma unroll
-        for (int k = 0; k < TL * NG; ++k) {
-            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&vp[k / NG][k % NG]));
+        for (int g = 0; g < NG; ++g) {
+            const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&vp[g]));
             const float m = fmaf(8.f, v.x, v.y);
-            wide[(lane + 32 * (k / NG)) * S::WIDE_LD + k % NG] = make_float4(v.x, v.x, m, m);
+            wide[lane * S::WIDE_LD + g] = make_float4(v.x, v.x, m, m);
         }
         __syncwarp();
 
@@ -605,7 +603,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
             l[t][h] = over_tokens(l[t][h]);
             if (i == 0) {
                 // (a row whose every score is NaN has no maximum, but is not empty)
-                xml[2 * (row + h)] = l[t][h] != l[t][h] && top[t][h] == -INFINITY ? 0.f : top[t][h] + e;
+                xml[2 * (row + h)] = l[t][h] != l[t][h] && top[t][h] == -INFINITY ? 0.f : top[t][h];
                 xml[2 * (row + h) + 1] = l[t][h];
             }
         }
@@ -766,8 +764,9 @@ int launch_att(const AttArgs& a, cudaStream_t stream) {
         attr_set[dev] = true;
     }
     const dim3 grid(a.splits, a.tiles * a.c.nkv, a.batch);
-    // (clusters up to 8: 2 x 64 queries over 1025 tokens 13.4 us, 14.7 with the second kernel; of 13 blocks they
-    // found no places: 4 x 32768 tokens 78 us for 56)
+    // Clusters of up to 4 / of up to 8 / the second kernel always, in us: 1 x 512 tokens, 12 heads 4.6 / 4.8 / 5.5;
+    // 8 x 1024 8.2 / 8.8 / 9.3; 16 x 2000 18.1 / 18.4 / 19.1; 2 x 64 queries over 1025 tokens 13.6 / 12.8 / 13.7.  (Of
+    // 13 blocks they found no places: 4 x 32768 tokens 78 for 56.)
     if (a.splits == 1 || a.splits > MAX_CLUSTER)
         return launch_kernel(kern, grid, dim3(THREADS), Shape<NG, NT>::TOTAL, stream, a) == cudaSuccess ? ET_OK : ET_ERR_CUDA;
     cudaLaunchConfig_t cfg = {};
@@ -812,7 +811,7 @@ int et_attention_kv4_fwd(const et_kv4_t* cache, const et_half* Q, et_half* Z, co
     if (mask_kind != ET_MASK_NONE && mask_kind != ET_MASK_CAUSAL && mask_kind != ET_MASK_ADDITIVE)
         return ET_ERR_INVALID_ARG;
     if (mask_kind == ET_MASK_ADDITIVE && (!mask || ldm < max_len)) return ET_ERR_INVALID_ARG;
-    if (!(scale > 0.f) || !(scale < INFINITY)) return ET_ERR_INVALID_ARG;
+    if (!(scale >= 0x1p-64f && scale <= 0x1p64f)) return ET_ERR_INVALID_ARG;  // (masks are divided by it)
     if (static_cast<int64_t>(table_ld) << a.c.page_shift < max_len) return ET_ERR_SHAPE;
     if (ldq % 8 || ldz % 8 || ldq < static_cast<int64_t>(nhead) * a.c.dh[0] || ldz < static_cast<int64_t>(nhead) * a.c.dh[1])
         return ET_ERR_SHAPE;

@@ -336,6 +336,55 @@ def test_attention_masked_nan_does_not_reach_the_output(et, cuda):
     assert bool(torch.isnan(z[0, :64]).all()) and bool(torch.isfinite(z[0, 64:]).all())
 
 
+@pytest.mark.parametrize("mask_kind", [1, 3], ids=["causal", "additive"])
+@pytest.mark.parametrize("dh", [32, 64, 128])
+def test_attention_hidden_giants_cost_nothing(et, cuda, dh, mask_kind):
+    """Tokens with huge V that a row does not see, or whose weight is next to nothing, leave the row's precision
+    alone.  The output's own rounding is at most 2^-11 of each value, so of the norm, and 0.42 of that on the
+    whole; the remaining half covers the sums (2^-22 and less of the largest term each)."""
+    import torch
+    rng = _rng(dh + mask_kind)
+    seq, length, heads = 8, 300, 2
+    cache = et.KV4Cache(20, 16, heads, dh, dh, device=cuda)
+    table = _dev(np.arange(20, dtype=np.int32)[None], cuda)
+    k = rng.normal(0, 1, (length, heads * dh)).astype(np.float16)
+    v = rng.normal(0, 1, (length, heads * dh)).astype(np.float16)
+    giants = np.zeros(length, bool)
+    mask = np.zeros((seq, 304), np.float16)
+    if mask_kind == 1:
+        giants[-seq + 1:] = True  # the first query sees none of them
+        rows = [0]
+    else:
+        giants[rng.permutation(length)[:40]] = True
+        mask[:, :length][:, giants] = -np.inf
+        unlikely = np.flatnonzero(giants)[:20]
+        mask[:4, unlikely] = -60.0  # seen, with e^-60 of the weight
+        rows = list(range(seq))
+    v = np.clip(v.astype(np.float32) * np.where(giants, 15000, 1)[:, None], -60000, 60000).astype(np.float16)
+    q = rng.normal(0, 1, (seq, heads * dh)).astype(np.float16)
+    et.kv4_write(cache, _dev(k, cuda), _dev(v, cuda), table, None, 1, length)
+    z = et.attention_kv4(cache, _dev(q, cuda), table, _dev(np.array([length], np.int32), cuda), 1, seq, heads,
+                         max_len=length, mask_kind=mask_kind, mask=_dev(mask, cuda) if mask_kind == 3 else None)
+    assert et.device_error() == 0
+    z = z.cpu().numpy().astype(np.float64)
+    plain = [ref.values(*ref.quantise(x.reshape(length, heads, dh), 32)) for x in (k, v)]
+    limit = length - seq + 1 + np.arange(seq) if mask_kind == 1 else np.full(seq, length)
+    for h in range(heads):
+        at = slice(h * dh, (h + 1) * dh)
+        want = ref.attention(q[:, at].astype(np.float64), plain[0][:, h], plain[1][:, h], limit, dh ** -0.5,
+                             mask[:, :length].astype(np.float64) if mask_kind == 3 else None)
+        for r in rows:
+            off = np.linalg.norm(z[r, at] - want[r]) / np.linalg.norm(want[r])
+            assert off <= 2.0 ** -11, (h, r, off)
+
+
+@pytest.mark.parametrize("case", [(1, 40, 64, 1, 64, 64, 1024, [500]), (3, 1, 96, 3, 32, 128, 2048, [2049, 1, 4096]),
+                                  (1, 200, 2, 2, 128, 128, 16, [201]), (2, 2, 4, 4, 16, 16, 16, [513, 1024]),
+                                  (200, 1, 2, 1, 64, 64, 16, list(range(1, 201)))], ids=str)
+def test_attention_many_rows_large_pages_large_batches(et, cuda, case):
+    _check_attention(et, cuda, *case, seed=17)
+
+
 def test_attention_shared_pages_streams_and_replays(et, cuda):
     """A prefix shared by all sequences; two streams at once; a captured call replayed with other lengths, beside
     eager ones."""

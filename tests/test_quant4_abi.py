@@ -85,7 +85,8 @@ def test_attention_refuses(et):
                     (dict(nhead=6), -3), (dict(nhead=0), -1), (dict(ldq=504), -3), (dict(ldz=510), -3),
                     (dict(max_len=65), -3), (dict(kind=2), -1), (dict(kind=7), -1), (dict(kind=3), -1),
                     (dict(kind=3, mask=0x9000, ldm=63), -1), (dict(scale=0.0), -1), (dict(scale=nan), -1),
-                    (dict(scale=inf), -1), (dict(scale=-1.0), -1), (dict(Q=0x5004), -2), (dict(Z=0x6008), -2),
+                    (dict(scale=inf), -1), (dict(scale=1e-30), -1), (dict(scale=1e30), -1),
+                    (dict(scale=-1.0), -1), (dict(Q=0x5004), -2), (dict(Z=0x6008), -2),
                     (dict(batch=65536), -3), (dict(seq=1 << 22, batch=1), -3),
                     (dict(table_ld=4096, max_len=65536, ws=None), -6),
                     (dict(table_ld=4096, max_len=65536, bytes=64), -6),
