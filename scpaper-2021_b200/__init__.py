@@ -370,6 +370,13 @@ def _require(name: str, dtype, *tensors) -> None:
             raise EtError(f"{name}: the values of a row must be contiguous")
 
 
+def _scratch_bytes(name: str, t) -> int:
+    """Size of a workspace, which must be contiguous and on the current device."""
+    if t.get_device() != _torch_c()._cuda_getDevice() or not t.is_contiguous():
+        raise EtError(f"{name}: a contiguous workspace on the current device is wanted")
+    return t.numel() * t.element_size()
+
+
 def _row_stride(t, width: int) -> int:
     """Stride of a matrix's rows (a single row may report any)."""
     if t.is_contiguous():
@@ -602,6 +609,8 @@ class KV4Cache:
         key = (batch, seq, nhead, max_len)
         n = self._workspace_bytes.get(key)
         if n is None:
+            if len(self._workspace_bytes) >= 256:  # (a max_len that grows with every token)
+                self._workspace_bytes.clear()
             n = self._workspace_bytes[key] = int(lib().et_attention_kv4_workspace_bytes(self._at, *key))
         return n
 
@@ -610,8 +619,8 @@ def _check_pages(name: str, cache: "KV4Cache", batch: int, table, *lengths) -> N
     _require(name, _types()[1], table, *lengths)
     if cache.device_index != table.get_device():
         raise EtError(f"{name}: the cache is on {cache.k_codes.device}")
-    if table.dim() != 2 or table.shape[0] != batch:
-        raise EtError(f"{name}: a page table [{batch}, pages] is wanted")
+    if table.dim() != 2 or table.shape[0] != batch or not table.is_contiguous():  # (its width is its reach)
+        raise EtError(f"{name}: a contiguous page table [{batch}, pages] is wanted")
     for n in lengths:
         if n is not None and (n.numel() != batch or not n.is_contiguous()):
             raise EtError(f"{name}: one length per sequence ({batch}) is wanted")
@@ -630,7 +639,8 @@ def kv4_write(cache: "KV4Cache", k, v, table, start, batch: int, seq: int, new_l
     _check_rows("kv4_write", "k", k, batch * seq, cache.k_width)
     _check_rows("kv4_write", "v", v, batch * seq, cache.v_width)
     _call("et_kv4_write_fwd", cache._at, k.data_ptr(), v.data_ptr(), _row_stride(k, cache.k_width),
-          _row_stride(v, cache.v_width), table.data_ptr(), _row_stride(table, table.shape[1]), _a(start), _a(new_len), batch, seq, _raw_stream())
+          _row_stride(v, cache.v_width), table.data_ptr(), table.shape[1], _a(start), _a(new_len), batch,
+          seq, _raw_stream())
 
 
 def kv4_read(cache: "KV4Cache", table, batch: int, seq: int, start=None, length=None, out=None):
@@ -647,7 +657,8 @@ def kv4_read(cache: "KV4Cache", table, batch: int, seq: int, start=None, length=
         _check_rows("kv4_read", "k", k, rows, cache.k_width)
         _check_rows("kv4_read", "v", v, rows, cache.v_width)
     _call("et_kv4_read_fwd", cache._at, k.data_ptr(), v.data_ptr(), _row_stride(k, cache.k_width),
-          _row_stride(v, cache.v_width), table.data_ptr(), _row_stride(table, table.shape[1]), _a(start), _a(length), batch, seq, _raw_stream())
+          _row_stride(v, cache.v_width), table.data_ptr(), table.shape[1], _a(start), _a(length), batch,
+          seq, _raw_stream())
     return k, v
 
 
@@ -680,9 +691,8 @@ def attention_kv4(cache: "KV4Cache", q, table, kv_len, batch: int, seq: int, nhe
         if n:
             workspace = q.new_empty((n + 1) // 2)
     else:
-        n = workspace.numel() * workspace.element_size()
-    _call("et_attention_kv4_fwd", cache._at, q.data_ptr(), z.data_ptr(), table.data_ptr(),
-          _row_stride(table, table.shape[1]), kv_len.data_ptr(), _a(q_len), batch, seq, nhead,
+        n = _scratch_bytes("attention_kv4", workspace)
+    _call("et_attention_kv4_fwd", cache._at, q.data_ptr(), z.data_ptr(), table.data_ptr(), table.shape[1], kv_len.data_ptr(), _a(q_len), batch, seq, nhead,
           _row_stride(q, nhead * cache.dh_qk), _row_stride(z, nhead * cache.dh_v), max_len, mask_kind, _a(mask),
           ldm, cache.scale if scale is None else scale, _a(workspace), n, _raw_stream())
     return z
@@ -867,8 +877,8 @@ class EncoderLayer:
         if not x.is_contiguous() or not out.is_contiguous():
             raise EtError("forward_cached: contiguous x and out are wanted")
         _call("et_encoder_layer_cached_fwd", ctypes.addressof(self.desc), cache._at, _a(x), _a(out), batch, seq,
-              _a(table), _row_stride(table, table.shape[1]), _a(start), _a(kv_len), _a(new_len), max_len, _a(workspace),
-              workspace.numel() * workspace.element_size(), _raw_stream())
+              _a(table), table.shape[1], _a(start), _a(kv_len), _a(new_len), max_len, _a(workspace),
+              _scratch_bytes("forward_cached", workspace), _raw_stream())
         return out
 
 
@@ -1251,7 +1261,8 @@ class EncoderStack:
 class CachedStack:
     """N chained encoder layers (causal) that keep what they have seen: every layer has a 4-bit key/value cache
     for `batch` sequences of up to `max_len` tokens.  forward() takes the next tokens of all sequences - a whole
-    prompt, then one token at a time - and returns their outputs; reset() starts over.  Lengths live on the
+    prompt, then one token at a time - and returns their outputs; reset() starts over.  Every `seq` that has been
+    used keeps its buffers (a captured call needs them): pad prompts to a few lengths.  Lengths live on the
     device, so a captured forward() can be replayed for token after token (the caller then counts them: a token
     past max_len is dropped and reported by device_error() as 601)."""
 
@@ -1289,19 +1300,29 @@ class CachedStack:
                 for _ in range(2)])
         return got
 
-    def forward(self, x, seq: int, new_len=None):
-        """x [batch * seq, hidden]: `seq` new tokens of every sequence, of which new_len[b] (int32) count.  The
-        result is overwritten by the next call with the same `seq`."""
-        if self.used + seq > self.max_len:
-            raise EtError(f"CachedStack: {self.used} + {seq} tokens do not fit into {self.max_len}")
+    def forward(self, x, seq: int, new_len=None, longest=None):
+        """x [batch * seq, hidden]: `seq` new tokens of every sequence, of which new_len[b] (int32) count; longest:
+        the largest new_len, for the host's count (seq where None).  The result is overwritten by the next call
+        with the same `seq`, which may have it for its x."""
+        longest = seq if longest is None else longest
+        if seq <= 0 or not 0 <= longest <= seq:
+            raise EtError(f"CachedStack: {longest} of {seq} new tokens")
+        if self.used + longest > self.max_len:
+            raise EtError(f"CachedStack: {self.used} + {longest} tokens do not fit into {self.max_len}")
+        # (all of it before the lengths move)
+        _require("CachedStack", _types()[0], x)
+        _check_rows("CachedStack", "x", x, self.batch * seq, self.layers[0].hidden)
+        _check_pages("CachedStack", self.caches[0], self.batch, self.table, new_len)
+        if not x.is_contiguous():
+            raise EtError("CachedStack: a contiguous x is wanted")
         ws, buf = self._buffers_of(seq)
         self.start.copy_(self.kv_len)
-        self.kv_len.add_(seq if new_len is None else new_len)
+        self.kv_len.add_(seq if new_len is None else new_len.reshape(-1).clamp(0, seq))
         cur = x
         for i, (layer, cache) in enumerate(zip(self.layers, self.caches)):
             cur = layer.forward_cached(cur, buf[i & 1], cache, self.table, self.start, self.kv_len, self.batch, seq,
                                        self.max_len, ws, new_len)
-        self.used += seq
+        self.used += longest
         return cur
 
 

@@ -221,6 +221,13 @@ int check_layer(const et_encoder_layer_t* L) {
     if (L->ffn2.in != L->ff || L->ffn2.out != L->hidden) return ET_ERR_SHAPE;
     if (!L->ln1_gamma || !L->ln1_beta || !L->ln2_gamma || !L->ln2_beta) return ET_ERR_INVALID_ARG;
     if (L->act != ET_ACT_RELU && L->act != ET_ACT_GELU) return ET_ERR_INVALID_ARG;
+    for (const et_linear_t* l : {&L->qkv, &L->o, &L->ffn1, &L->ffn2}) {
+        if (l->format != ET_FMT_W4) continue;
+        size_t codes, params;
+        const int st = et_w4_sizes(l->in, l->out, l->nnz_tiles, &codes, &params);
+        if (st != ET_OK) return st;
+        if (!l->weight || !l->row_ptr) return ET_ERR_INVALID_ARG;
+    }
     return ET_OK;
 }
 

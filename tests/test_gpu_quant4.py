@@ -385,6 +385,55 @@ def test_attention_many_rows_large_pages_large_batches(et, cuda, case):
     _check_attention(et, cuda, *case, seed=17)
 
 
+def test_calls_that_share_a_position_or_a_scratch(et, cuda):
+    """A position named by several rows keeps the codes of one of them or a mixture (nothing else is touched); a
+    given workspace is used, and one on the host, or a page table with gaps between its rows, is refused."""
+    import torch
+    rng = _rng(18)
+    cache = et.KV4Cache(40, 16, 1, 64, 64, device=cuda)
+    twice = _dev(np.array([[3, 4], [3, 5]], np.int32), cuda)
+    same = rng.normal(0, 1, (32, 64)).astype(np.float16)
+    x = _dev(np.concatenate([same, same]), cuda)
+    for t in (cache.k_codes, cache.k_params, cache.v_codes, cache.v_params):
+        t.zero_()
+    et.kv4_write(cache, x, x, twice, None, 2, 32)
+    k, _ = et.kv4_read(cache, twice, 2, 32)
+    assert torch.equal(k[:32], k[32:])
+    assert not cache.k_codes[:3].any() and not cache.k_codes[6:].any()
+    table = _dev(np.arange(36, dtype=np.int32)[None], cuda)
+    x = _dev(rng.normal(0, 1, (576, 64)).astype(np.float16), cuda)
+    et.kv4_write(cache, x, x, table, None, 1, 576)
+    q = x[:8]
+    n = _dev(np.array([576], np.int32), cuda)
+    need = cache.workspace_bytes(1, 8, 1, 576)
+    want = et.attention_kv4(cache, q, table, n, 1, 8, 1)
+    ws = torch.full((max(need, 16),), 255, dtype=torch.uint8, device=cuda)
+    assert torch.equal(et.attention_kv4(cache, q, table, n, 1, 8, 1, workspace=ws), want)
+    gaps = torch.zeros((2, 40), dtype=torch.int32, device=cuda)[:, 4:20]
+    two = _dev(np.array([10, 10], np.int32), cuda)
+    xx = x[:16]
+    layer = et.EncoderLayer({k: np.asarray(v, np.float16) for k, v in _weights(et, 3, 64, 64).items()}, 1, et.ACT_GELU)
+    scratch = torch.empty(layer.cached_workspace_bytes(cache, 2, 1, 32), dtype=torch.uint8, device=cuda)
+    out = torch.empty_like(x[:2])
+    for f in (lambda: et.attention_kv4(cache, q, table, n, 1, 8, 1, workspace=ws.cpu()),
+              lambda: et.attention_kv4(cache, q[:2], gaps, two, 2, 1, 1),
+              lambda: et.kv4_write(cache, xx, xx, gaps, None, 2, 8),
+              lambda: et.kv4_read(cache, gaps, 2, 8),
+              lambda: layer.forward_cached(x[:2], out, cache, gaps, two, two, 2, 1, 32, scratch),
+              lambda: layer.forward_cached(x[:2], out, cache, twice, two, two, 2, 1, 32, scratch.cpu()),
+              lambda: layer.forward_cached(x[:2], out, cache, twice, two, two, 2, 1, 32, scratch[:256])):
+        with pytest.raises(et.EtError):
+            f()
+    assert et.device_error() == 0
+
+
+def test_workspace_sizes_do_not_pile_up(et, cuda):
+    cache = et.KV4Cache(4, 16, 2, 64, 64, device=cuda)
+    for n in range(1, 2000):
+        cache.workspace_bytes(1, 1, 2, n)
+    assert len(cache._workspace_bytes) <= 256
+
+
 def test_attention_shared_pages_streams_and_replays(et, cuda):
     """A prefix shared by all sequences; two streams at once; a captured call replayed with other lengths, beside
     eager ones."""
@@ -713,3 +762,59 @@ def test_cached_stack_answers_token_by_token(et, cuda):
     with pytest.raises(et.EtError):
         stack.used = total
         stack.forward(step, 1)
+
+
+def test_cached_stack_refuses_before_its_lengths_move(et, cuda):
+    import torch
+    hidden, batch = 128, 2
+    layers = [et.EncoderLayer({k: np.asarray(v, np.float16) for k, v in _weights(et, 51, hidden, 256).items()}, 2,
+                              et.ACT_GELU)]
+    stack = et.CachedStack(layers, batch, 33, page=16, device=cuda)
+    x = _dev(_rng(19).normal(0, 1, (batch * 6, hidden)).astype(np.float16), cuda)
+    want = stack.forward(x, 6).clone()
+    stack.reset()
+    n = _dev(np.array([6, 6], np.int32), cuda)
+    for f in (lambda: stack.forward(x.float(), 6), lambda: stack.forward(x, 5), lambda: stack.forward(x[:, :64], 6),
+              lambda: stack.forward(x, 6, new_len=n.long()), lambda: stack.forward(x, 6, new_len=n[:1]),
+              lambda: stack.forward(x.cpu(), 6), lambda: stack.forward(x, 6, longest=7), lambda: stack.forward(x, 0),
+              lambda: stack.forward(x.t().contiguous().t(), 6)):
+        with pytest.raises(et.EtError):
+            f()
+        assert not bool(stack.kv_len.any()) and stack.used == 0
+    assert torch.equal(stack.forward(x, 6), want)
+    # lengths past the rows count the rows; the result may be the next call's input
+    stack.reset()
+    got = stack.forward(x, 6, new_len=n + 100)
+    assert torch.equal(got, want) and stack.kv_len.tolist() == [6, 6]
+    again = stack.forward(got, 6).clone()
+    stack.reset()
+    stack.forward(x, 6)
+    assert torch.equal(stack.forward(want.clone(), 6), again)
+    # padded rows do not use up the host's count where `longest` tells it
+    stack.reset()
+    short = _dev(np.array([2, 1], np.int32), cuda)
+    for _ in range(16):
+        stack.forward(x, 6, new_len=short, longest=2)
+    assert stack.used == 32 and stack.kv_len.tolist() == [32, 16] and et.device_error() == 0
+    with pytest.raises(et.EtError):
+        stack.forward(x, 6, new_len=short, longest=2)
+
+
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("batch,seq", [(1, 5), (2, 100)])
+def test_layer_and_stack_of_4_bit_weights(et, cuda, group, batch, seq):
+    """The whole-sequence layer with 4-bit weights against the dense layer of the weights that they stand for (which
+    differ from them by their rounding to fp16)."""
+    from conftest import assert_close
+    hidden, ff, nhead = 256, 512, 4
+    names = ("wqkv", "wo", "w1", "w2")
+    w = {k: np.asarray(v, np.float16) for k, v in _weights(et, 61, hidden, ff).items()}
+    plain = dict(w)
+    for n in names:
+        plain[n] = et.W4Weight(_dev(w[n], cuda), group).densify().cpu().numpy()
+    x = _dev(_rng(20).normal(0, 1, (batch * seq, hidden)).astype(np.float16), cuda)
+    stacks = [et.EncoderStack([et.EncoderLayer(a, nhead, et.ACT_GELU, formats=f) for _ in range(2)], batch, seq,
+                              device=cuda) for a, f in ((w, {n: ("w4", group) for n in names}), (plain, None))]
+    got, want = (s.forward(x, et.MASK_CAUSAL).cpu().numpy() for s in stacks)
+    assert et.device_error() == 0
+    assert_close(got, want, "stack")

@@ -173,6 +173,13 @@ def test_cached_layer_refuses(et):
                                                P(kv), None, most, P(ws), Z(n), None)
 
     assert fwd(table=None) == -1 and fwd(most=65) == -3
+    # 4-bit weights that no kernel takes are found before the first launch
+    keep = d.ffn2.format
+    d.ffn2.format, d.ffn2.row_ptr, d.ffn2.nnz_tiles = et.FMT_W4, 0x700000, 48
+    assert fwd() == -3
+    d.ffn2.nnz_tiles, d.ffn2.row_ptr = 64, None
+    assert fwd() == -1
+    d.ffn2.format, d.ffn2.nnz_tiles = keep, 0
 
     assert fwd(x=None) == -1 and fwd(start=None) == -1 and fwd(kv=None) == -1
     assert fwd(ws=None) == -6 and fwd(n=need - 1) == -6
