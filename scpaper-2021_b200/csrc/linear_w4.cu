@@ -13,6 +13,10 @@
 // thread block share 1, 2 or 4 panels of 16 rows and split the features among them, adding up in shared
 // memory; a block walks panels until none is left.  Activations are staged in shared memory, in chunks when
 // they do not fit.  Weights do not depend on earlier kernels: the ring is filled before the wait for them.
+//
+// What bounds it.  8192 -> 8192, one token: 9.8 us, 35.7 MB at 3.6 TB/s - 3 us of launch, filling of the rings and
+// joining of the warps, then about 5.3 TB/s.  768 -> 2304: 2.4 us, all of it latency.  Loads into registers instead of the
+// rings took 13.6 us.
 #include <atomic>
 
 #include "kernels.h"
