@@ -184,8 +184,8 @@ struct PackedExpander {
 // written.  A code becomes fp16 exactly (1024 + c, less 1024), and c s + m is rounded to fp16 once: the tensor
 // core cannot scale its sums per group, so the operand has to carry the scale.  Lane 4 i + j expands the four
 // words of rows i and i + 8.  Blocks are copied asynchronously QUANT_AHEAD ahead into a ring of the warp's own (64 tokens
-// x 8192 -> 8192: 32 us; loads into registers, which are waited for together with younger ones, 33).  A K block
-// of 64 takes 0.24 us, whatever is expanded: the one thread that issues the products and their commits bounds it.
+// x 8192 -> 8192: 32 us; loads into registers, which are waited for together with younger ones, 33).  What
+// bounds it: quant_cycles below.
 constexpr int QUANT_AHEAD = 4;
 constexpr int QUANT_BLOCK = 1024 + 256;  // codes, and (s, m) of 16 rows x up to four groups
 struct QuantExpander {
@@ -689,6 +689,16 @@ struct ExpandPlan {
     long panels, waves, cycles;
 };
 
+// 4 bits: cycles of a K block for mb token blocks, fitted to B200 runs: 8192 -> 8192 at 64 features took 466 and 677
+// for one and two, at 128 features 690 (of expanding: 250 + 3.45 a feature), 916 and, for four, 1490: the thread that
+// issues products and commits bounds a block as long as there are several, the expansion where there is one.  (By the
+// products' 256 cycles alone, as the other formats are planned, 2000 tokens 8192 -> 8192 took 356 us for 225, 8192
+// tokens 4096 -> 4096 271 for 239.)
+long quant_cycles(int bn, int mb) {
+    const long products = bn == 128 ? 342 + 287 * mb : 255 + 211 * mb, expand = 250 + bn * 7 / 2;
+    return products > expand ? products : expand;
+}
+
 // Fills in a.mb, a.groups, a.ckb, a.nbuf and a.na.
 template <int FMT>
 ExpandPlan plan_expand(ExpandArgs& a) {
@@ -709,7 +719,8 @@ ExpandPlan plan_expand(ExpandArgs& a) {
     for (int mb = 1; mb <= mb_max && mb <= tblocks; ++mb) {
         const long groups = (tblocks + mb - 1) / mb;
         const long waves = (panels(bn) * groups + sms - 1) / sms;
-        const long cost = waves * (4000 + static_cast<long>(mb) * (nkb * (bn == 128 ? 256 : 240) + 600));
+        const long per = FMT == FMT_QUANT ? quant_cycles(bn, mb) : static_cast<long>(mb) * (bn == 128 ? 256 : 240);
+        const long cost = waves * (4000 + nkb * per + 600l * mb);
         if (best < 0 || cost < best) {
             best = cost;
             best_waves = waves;
@@ -790,15 +801,13 @@ int launch_linear_expand_packed(const uint32_t* pk_mask, const int* pk_off, cons
     return launch_expand<FMT_PACKED>(a, stream);
 }
 
-// Every K block of a CTA's token block costs one thread four products and their completion, 0.24 us whatever the
-// panel's width.
 double linear_expand_w4_us(int T, int in, int out) {
     ExpandArgs a = {};
     a.T = T;
     a.in = in;
     a.out = out;
     const ExpandPlan p = plan_expand<FMT_QUANT>(a);
-    return 1.7 + 0.24 * ((in + BK - 1) / BK) * p.waves * a.mb;
+    return 1.5 + quant_cycles(p.bn, a.mb) / 1850.0 * ((in + BK - 1) / BK) * p.waves;
 }
 
 int launch_linear_expand_w4(const uint8_t* codes, const __half* params, int group, const __half* bias,
