@@ -14,10 +14,10 @@
 // too unlikely to count, costs it no precision.
 //
 // A thread block owns up to 16 query rows that share a key/value head (the heads of a group times the query
-// tokens) and a chunk of the sequence; its four warps take 32-token tiles in turn, each with a ring of asynchronous
-// copies of its own (page contents land in shared memory as they are; no thread waits for another warp in the
-// loop).  With few rows the sequence is split over the blocks of a cluster, which join their partial results
-// through distributed shared memory, or (more than 4) over blocks that leave them to a second kernel.
+// tokens); its four warps take 32-token tiles in turn, each with a ring of asynchronous copies of its own (page
+// contents land in shared memory as they are; no thread waits for another warp in the loop).  With few rows the
+// sequence's tiles are dealt out to the blocks of a cluster, which join their partial results through distributed
+// shared memory, or (more than 4) to blocks that leave them to a second kernel.
 //
 // Layout.  Both products have the cache as their 16-row operand and eight query rows as their 8-column one: a few
 // rows then waste little of the tensor core and of the registers (with the rows on the 16 side, half
@@ -38,7 +38,7 @@ constexpr int WARPS = 4;
 constexpr int THREADS = 32 * WARPS;
 constexpr int MAX_SPLITS = 64;
 constexpr int JOIN_AHEAD = 16;  // partial results that the second kernel has in flight
-constexpr int MIN_CHUNK = 256;  // tokens of a split at least: two tiles per warp
+constexpr int MIN_CHUNK = 256;  // tokens of max_len to a split at least: two tiles per warp
 constexpr int MAX_CLUSTER = 4;  // splits that join through distributed shared memory
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -54,7 +54,7 @@ struct AttArgs {
     float* part_ml;
     int table_ld, batch, seq, nhead, ratio, ldq, ldz, ldm, max_len, mask_kind;
     int tiles;        // of query rows per (sequence, key/value head)
-    int splits, per;  // blocks along the sequence, tokens of each
+    int splits;       // blocks along the sequence
     FastDiv by_ratio;
     float scale_log2;
     int* err_word;
@@ -217,12 +217,13 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
             qf[g][t][0] = v.x, qf[g][t][1] = v.y, qf[g][t][2] = v.z, qf[g][t][3] = v.w;
         }
     }
-    // Page numbers, of 16 tokens to a lane, BATCH tiles at a time; the warp's tiles are warp, warp + 4, ... of the
-    // block's chunk.  What the table holds past the sequence's end is read, but neither followed nor reported.
+    // The warps of a sequence's blocks take its tiles in turn: shares are even whatever its length, and known before
+    // it.  Page numbers: of 16 tokens to a lane, BATCH tiles at a time.  What the table holds past the sequence's end is
+    // read, but neither followed nor reported.
     constexpr int BATCH = 32 / HALVES;
-    const int first = split * a.per;
+    const int turn = split * WARPS + warp, turns = a.splits * WARPS;  // the warp's tiles: turn, turn + turns, ...
     const int* table = a.table + static_cast<int64_t>(b) * a.table_ld;
-    auto position = [&](int n) { return first + ((n + lane / HALVES) * WARPS + warp) * TILE + lane % HALVES * 16; };
+    auto position = [&](int n) { return ((n + lane / HALVES) * turns + turn) * TILE + lane % HALVES * 16; };
     auto entry = [&](int n) {
         const int pos = position(n), e = pos >> a.c.page_shift;
         return pos < a.max_len && e < a.table_ld ? __ldcg(table + e) : -1;
@@ -236,20 +237,19 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
     len = len < 0 ? 0 : len;
     nq = nq < 0 ? 0 : (nq > a.seq ? a.seq : nq);
     if (row0 >= nq * a.ratio) return;  // (rows are ordered by query token)
-    int most, least;  // the largest and smallest number of tokens that a row sees: the last and first row's
+    int end, least;  // the largest and smallest number of tokens that a row sees: the last and first row's
     {
         const int last = (row0 + 8 * NT < nq * a.ratio ? row0 + 8 * NT : nq * a.ratio) - 1;
         if (a.mask_kind == ET_MASK_CAUSAL) {
             least = len - nq + static_cast<int>(a.by_ratio.div(row0)) + 1;
-            most = len - nq + static_cast<int>(a.by_ratio.div(last)) + 1;
+            end = len - nq + static_cast<int>(a.by_ratio.div(last)) + 1;
         } else {
-            least = most = len;
+            least = end = len;
         }
-        most = most < 0 ? 0 : most;
+        end = end < 0 ? 0 : end;
     }
-    const int end = first + a.per < most ? first + a.per : most;  // of this block's chunk
-    const int ntile = end > first ? (end - first + TILE - 1) / TILE : 0;
-    const int mine = ntile > warp ? (ntile - warp + WARPS - 1) / WARPS : 0;
+    const int ntile = (end + TILE - 1) / TILE;
+    const int mine = ntile > turn ? (ntile - turn + turns - 1) / turns : 0;
     auto checked = [&](int n, int id) {  // page of the lane's 16 tokens, or -1: nothing to read
         if (position(n) >= end || n + lane / HALVES >= mine) return -1;
         if (id >= 0 && id < a.c.num_pages) return id;
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
                 pages_next = checked(n + BATCH, entry(n + BATCH));
             }
             const uint32_t st = ring32 + (n % STAGES) * S::STAGE;
-            const int pos = first + (n * WARPS + warp) * TILE;
+            const int pos = (n * turns + turn) * TILE;
 #pragma unroll
             for (int h = 0; h < HALVES; ++h) {
                 const int id = __shfl_sync(0xffffffffu, pages, n % BATCH * HALVES + h);
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
         __syncwarp();
         issue(n + STAGES - 1);  // into the slot that the previous tile left
         const uint8_t* st = ring + (n % STAGES) * S::STAGE;
-        const int tok0 = first + (n * WARPS + warp) * TILE;
+        const int tok0 = (n * turns + turn) * TILE;
 
         // ---- the lane's token: K's (s, m) to fp32; V's largest s, and whether all of V's are finite
         uint32_t vp[NG], odd_bits = 0, s_top = 0;
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
             uint32_t kp[NG];
             lds_words<NG>(st + 2 * S::CODES + lane * 4 * NG, kp);
             lds_words<NG>(st + 2 * S::CODES + S::PARAMS + lane * 4 * NG, vp);
-            if (tok0 + lane >= end) {  // not of this sequence, or this block's: counts as zeros
+            if (tok0 + lane >= end) {  // hidden from every row: counts as zeros
 #pragma unroll
                 for (int g = 0; g < NG; ++g) kp[g] = vp[g] = 0u;
             }
@@ -836,7 +836,6 @@ int et_attention_kv4_fwd(const et_kv4_t* cache, const et_half* Q, et_half* Z, co
     a.by_ratio = et::FastDiv(static_cast<uint32_t>(a.ratio));
     a.tiles = p.tiles;
     a.splits = p.splits;
-    a.per = ((max_len + p.splits - 1) / p.splits + 31) / 32 * 32;  // whole tiles
     a.scale_log2 = scale * et::LOG2E;
     a.err_word = et::device_error_word();
     if (!a.err_word) return ET_ERR_NO_DEVICE;
