@@ -264,6 +264,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
     const uint8_t* code_base[2] = {a.c.codes[0] + lane * 16, a.c.codes[1] + lane * 16};
     const uint8_t* param_base = reinterpret_cast<const uint8_t*>(a.c.params[lane >> 4]) + (lane & 15) * 16;
     const uint32_t param_at = 2 * S::CODES + (lane >> 4) * (S::PARAMS - 256);
+    int next_pos = turn * TILE;
     auto issue = [&](int n) {
         if (n < mine) {
             if (n != 0 && n % BATCH == 0) {
@@ -271,12 +272,11 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
                 pages_next = checked(n + BATCH, entry(n + BATCH));
             }
             const uint32_t st = ring32 + (n % STAGES) * S::STAGE;
-            const int pos = (n * turns + turn) * TILE;
 #pragma unroll
             for (int h = 0; h < HALVES; ++h) {
                 const int id = __shfl_sync(0xffffffffu, pages, n % BATCH * HALVES + h);
                 const int have = id < 0 ? 0 : 16;
-                const int64_t row = kv4_row(a.c, max(id, 0), pos + 16 * h, kvh);
+                const int64_t row = kv4_row(a.c, max(id, 0), next_pos + 16 * h, kvh);
 #pragma unroll
                 for (int of = 0; of < 2; ++of)
 #pragma unroll
@@ -288,6 +288,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
                     cp_async16(st + param_at + h * 64 * NG, param_base + row * (4 * NG), have);
             }
         }
+        next_pos += turns * TILE;
         cp_async_commit();  // (an empty group past the last tile, so that the count stays)
     };
 #pragma unroll
@@ -354,12 +355,12 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
     }
 
     const uint64_t minus_one = pack_f32x2(-1.f, -1.f);
-    for (int n = 0; n < mine; ++n) {
+    int tok0 = turn * TILE;
+    for (int n = 0; n < mine; ++n, tok0 += turns * TILE) {
         cp_async_wait<STAGES - 2>();
         __syncwarp();
         issue(n + STAGES - 1);  // into the slot that the previous tile left
         const uint8_t* st = ring + (n % STAGES) * S::STAGE;
-        const int tok0 = (n * turns + turn) * TILE;
 
         // ---- the lane's token: K's (s, m) to fp32; V's largest s, and whether all of V's are finite
         uint32_t vp[NG], odd_bits = 0, s_top = 0;
