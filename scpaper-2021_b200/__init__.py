@@ -185,14 +185,19 @@ _KINDS = {"p": c_void_p, "i": c_int, "z": c_size_t, "f": c_float}
 _calls = {}
 
 
-def _call(name: str, *args) -> None:
-    """One forward entry point with plain Python arguments; raises on a status."""
+def _entry(name: str):
+    """One forward entry point, to be called with plain Python arguments; returns its status."""
     fn = _calls.get(name)
     if fn is None or fn[0] is not _lib:
         proto = ctypes.CFUNCTYPE(c_int, *[_KINDS[k] for k in _SIGNATURES[name]])
         fn = (lib(), proto((name, lib())))
         _calls[name] = fn
-    status = fn[1](*args)
+    return fn[1]
+
+
+def _call(name: str, *args) -> None:
+    """The same, raising on a status (the shortest calls do without the detour of their arguments)."""
+    status = _entry(name)(*args)
     if status != 0:
         check(status, name)
 
@@ -411,7 +416,7 @@ class W4Weight:
         self.params = torch.empty(self.param_shape, dtype=torch.float16, device=w.device)
         _call("et_w4_pack", _a(w), inn, out, group, _a(self.codes), _a(self.params), _raw_stream())
         torch.cuda.current_stream().synchronize()  # weights must be complete before their first use
-        self.codes_at, self.params_at = self.codes.data_ptr(), self.params.data_ptr()
+        self._place()
 
     def _set(self, inn: int, out: int, group: int) -> None:
         code_bytes, param_bytes = c_size_t(0), c_size_t(0)
@@ -421,6 +426,10 @@ class W4Weight:
         self.inn, self.out, self.group = inn, out, group
         self.code_shape = (out // 16, nb, 2, 32, 16)
         self.param_shape = (out // 16, nb, 16, 128 // group, 2)
+
+    def _place(self) -> None:
+        self.codes_at, self.params_at = self.codes.data_ptr(), self.params.data_ptr()
+        self.device_index = self.codes.get_device()
 
     @classmethod
     def from_arrays(cls, codes, params, inn: int, out: int, group: int):
@@ -434,7 +443,7 @@ class W4Weight:
         if not codes.is_contiguous() or not params.is_contiguous():
             raise EtError("W4Weight: contiguous arrays are wanted")
         w.codes, w.params = codes, params
-        w.codes_at, w.params_at = codes.data_ptr(), params.data_ptr()
+        w._place()
         return w
 
     def densify(self):
@@ -452,19 +461,16 @@ def linear_w4(x, w: "W4Weight", bias=None, act=ACT_NONE, out=None):
     T, inn = x.shape
     if inn != w.inn or not x.is_contiguous():
         raise EtError(f"linear_w4: contiguous activations [T, {w.inn}] are wanted")
-    f16 = _types()[0]
-    if out is None:
-        y = x.new_empty((T, w.out))
-        _require("linear_w4", f16, x, bias)
-    else:
-        y = out
-        _require("linear_w4", f16, x, bias, y)
-        if y.shape != (T, w.out) or not y.is_contiguous():
-            raise EtError(f"linear_w4: a contiguous result [{T}, {w.out}] is wanted")
-    if w.codes.get_device() != x.get_device() or (bias is not None and bias.shape != (w.out,)):
+    y = x.new_empty((T, w.out)) if out is None else out
+    _require("linear_w4", _types()[0], x, bias, out)
+    if out is not None and (out.shape != (T, w.out) or not out.is_contiguous()):
+        raise EtError(f"linear_w4: a contiguous result [{T}, {w.out}] is wanted")
+    if w.device_index != x.get_device() or (bias is not None and bias.shape != (w.out,)):
         raise EtError(f"linear_w4: the weight's device and a bias [{w.out}] are wanted")
-    _call("et_linear_w4_fwd", w.codes_at, w.params_at, w.group, _a(bias), x.data_ptr(), y.data_ptr(), T, inn, w.out,
-          act, _raw_stream())
+    status = _entry("et_linear_w4_fwd")(w.codes_at, w.params_at, w.group, None if bias is None else bias.data_ptr(),
+                                        x.data_ptr(), y.data_ptr(), T, inn, w.out, act, _raw_stream())
+    if status != 0:
+        check(status, "et_linear_w4_fwd")
     return y
 
 
@@ -616,13 +622,19 @@ class KV4Cache:
 
 
 def _check_pages(name: str, cache: "KV4Cache", batch: int, table, *lengths) -> None:
-    _require(name, _types()[1], table, *lengths)
-    if cache.device_index != table.get_device():
+    i32, dev = _types()[1], cache.device_index
+    if dev != _torch_c()._cuda_getDevice():
         raise EtError(f"{name}: the cache is on {cache.k_codes.device}")
+    if table.dtype is not i32 or table.get_device() != dev:
+        _require(name, i32, table)
     if table.dim() != 2 or table.shape[0] != batch or not table.is_contiguous():  # (its width is its reach)
         raise EtError(f"{name}: a contiguous page table [{batch}, pages] is wanted")
     for n in lengths:
-        if n is not None and (n.numel() != batch or not n.is_contiguous()):
+        if n is None:
+            continue
+        if n.dtype is not i32 or n.get_device() != dev:
+            _require(name, i32, n)
+        if n.numel() != batch or not n.is_contiguous():
             raise EtError(f"{name}: one length per sequence ({batch}) is wanted")
 
 
@@ -638,9 +650,11 @@ def kv4_write(cache: "KV4Cache", k, v, table, start, batch: int, seq: int, new_l
     _check_pages("kv4_write", cache, batch, table, start, new_len)
     _check_rows("kv4_write", "k", k, batch * seq, cache.k_width)
     _check_rows("kv4_write", "v", v, batch * seq, cache.v_width)
-    _call("et_kv4_write_fwd", cache._at, k.data_ptr(), v.data_ptr(), _row_stride(k, cache.k_width),
-          _row_stride(v, cache.v_width), table.data_ptr(), table.shape[1], _a(start), _a(new_len), batch,
-          seq, _raw_stream())
+    status = _entry("et_kv4_write_fwd")(
+        cache._at, k.data_ptr(), v.data_ptr(), _row_stride(k, cache.k_width), _row_stride(v, cache.v_width),
+        table.data_ptr(), table.shape[1], _a(start), _a(new_len), batch, seq, _raw_stream())
+    if status != 0:
+        check(status, "et_kv4_write_fwd")
 
 
 def kv4_read(cache: "KV4Cache", table, batch: int, seq: int, start=None, length=None, out=None):
@@ -656,9 +670,11 @@ def kv4_read(cache: "KV4Cache", table, batch: int, seq: int, start=None, length=
         _require("kv4_read", f16, k, v)
         _check_rows("kv4_read", "k", k, rows, cache.k_width)
         _check_rows("kv4_read", "v", v, rows, cache.v_width)
-    _call("et_kv4_read_fwd", cache._at, k.data_ptr(), v.data_ptr(), _row_stride(k, cache.k_width),
-          _row_stride(v, cache.v_width), table.data_ptr(), table.shape[1], _a(start), _a(length), batch,
-          seq, _raw_stream())
+    status = _entry("et_kv4_read_fwd")(
+        cache._at, k.data_ptr(), v.data_ptr(), _row_stride(k, cache.k_width), _row_stride(v, cache.v_width),
+        table.data_ptr(), table.shape[1], _a(start), _a(length), batch, seq, _raw_stream())
+    if status != 0:
+        check(status, "et_kv4_read_fwd")
     return k, v
 
 
@@ -692,9 +708,12 @@ def attention_kv4(cache: "KV4Cache", q, table, kv_len, batch: int, seq: int, nhe
             workspace = q.new_empty((n + 1) // 2)
     else:
         n = _scratch_bytes("attention_kv4", workspace)
-    _call("et_attention_kv4_fwd", cache._at, q.data_ptr(), z.data_ptr(), table.data_ptr(), table.shape[1], kv_len.data_ptr(), _a(q_len), batch, seq, nhead,
-          _row_stride(q, nhead * cache.dh_qk), _row_stride(z, nhead * cache.dh_v), max_len, mask_kind, _a(mask),
-          ldm, cache.scale if scale is None else scale, _a(workspace), n, _raw_stream())
+    status = _entry("et_attention_kv4_fwd")(
+        cache._at, q.data_ptr(), z.data_ptr(), table.data_ptr(), table.shape[1], kv_len.data_ptr(), _a(q_len), batch, seq,
+        nhead, _row_stride(q, nhead * cache.dh_qk), _row_stride(z, nhead * cache.dh_v), max_len, mask_kind, _a(mask), ldm,
+        cache.scale if scale is None else scale, _a(workspace), n, _raw_stream())
+    if status != 0:
+        check(status, "et_attention_kv4_fwd")
     return z
 
 
