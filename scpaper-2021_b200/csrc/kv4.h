@@ -37,6 +37,7 @@ inline int kv4_view(const et_kv4_t* c, Kv4View& v, bool pointers) {
     v.num_pages = c->num_pages;
     v.page_shift = 0;
     while ((1 << v.page_shift) < c->page) ++v.page_shift;
+    if (static_cast<int64_t>(c->num_pages) * c->nkv > INT64_MAX >> (v.page_shift + 8)) return ET_ERR_SHAPE;  // (bytes)
     v.nkv = c->nkv;
     v.dh[0] = c->dh_qk;
     v.dh[1] = c->dh_v;

@@ -434,6 +434,51 @@ def test_workspace_sizes_do_not_pile_up(et, cuda):
     assert len(cache._workspace_bytes) <= 256
 
 
+@pytest.mark.parametrize("length", [60, 3000])
+def test_attention_query_that_is_not_finite_stays_in_its_row(et, cuda, length):
+    import torch
+    rng = _rng(23)
+    cache = et.KV4Cache(200, 16, 2, 64, 64, device=cuda)
+    table = _dev(np.arange(200, dtype=np.int32)[None], cuda)
+    x = _dev(rng.normal(0, 1, (length, 128)).astype(np.float16), cuda)
+    et.kv4_write(cache, x, x, table, None, 1, length)
+    q = rng.normal(0, 1, (3, 256)).astype(np.float16)
+    n = _dev(np.array([length], np.int32), cuda)
+    clean = et.attention_kv4(cache, _dev(q, cuda), table, n, 1, 3, 4)
+    q[1, 70], q[2, 3] = np.nan, np.inf  # heads 1 and 0
+    z = et.attention_kv4(cache, _dev(q, cuda), table, n, 1, 3, 4)
+    want = torch.zeros_like(z, dtype=torch.bool)
+    want[1, 64:128] = want[2, :64] = True
+    assert torch.equal(torch.isnan(z), want) and torch.equal(z[~want], clean[~want])
+
+
+def test_two_graphs_of_the_same_call(et, cuda):
+    """Each captured call has partial results of its own: replayed at once on two streams they do not meet."""
+    import torch
+    rng = _rng(24)
+    cache = et.KV4Cache(300, 16, 2, 64, 64, device=cuda)
+    table = _dev(np.arange(300, dtype=np.int32)[None], cuda)
+    x = _dev(rng.normal(0, 1, (4800, 128)).astype(np.float16), cuda)
+    et.kv4_write(cache, x, x, table, None, 1, 4800)
+    n = _dev(np.array([4700], np.int32), cuda)
+    assert cache.workspace_bytes(1, 1, 4, 4800) > 0
+    qs = [_dev(rng.normal(0, 1, (1, 256)).astype(np.float16), cuda) for _ in range(2)]
+    want = [et.attention_kv4(cache, q, table, n, 1, 1, 4).clone() for q in qs]
+    graphs, outs = [], []
+    for q in qs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(et.attention_kv4(cache, q, table, n, 1, 1, 4))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want)) and et.device_error() == 0
+
+
 def test_attention_shared_pages_streams_and_replays(et, cuda):
     """A prefix shared by all sequences; two streams at once; a captured call replayed with other lengths, beside
     eager ones."""

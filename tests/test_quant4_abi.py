@@ -30,6 +30,16 @@ def test_cache_sizes(et):
     assert et.lib().et_kv4_sizes(None, None, None) == -1
 
 
+def test_cache_whose_bytes_pass_64_bits_is_refused(et):
+    c = _cache(et, num_pages=2 ** 31 - 1, nkv=2 ** 21, page=2 ** 30)
+    a, b = Z(0), Z(0)
+    et.lib().et_kv4_sizes.argtypes = [P, P, P]
+    assert et.lib().et_kv4_sizes(ctypes.addressof(c), ctypes.byref(a), ctypes.byref(b)) == -3
+    c = _cache(et, num_pages=2 ** 31 - 1, nkv=1, page=16, dh_qk=128, dh_v=128)
+    assert et.lib().et_kv4_sizes(ctypes.addressof(c), ctypes.byref(a), ctypes.byref(b)) == 0
+    assert a.value == (2 ** 31 - 1) * 16 * 64
+
+
 def test_positions_outside_the_table_or_the_cache_are_not_followed(et):
     fn = et.lib().et_debug_kv4_row
     fn.restype, fn.argtypes = ctypes.c_longlong, [P, P, I, ctypes.c_longlong, I]
