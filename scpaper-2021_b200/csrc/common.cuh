@@ -493,6 +493,9 @@ __device__ __forceinline__ void cluster_sync_all() {
 __device__ __forceinline__ void cluster_arrive_relaxed() {
     asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
 }
+__device__ __forceinline__ void cluster_arrive() {  // orders what came before
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_wait() {
     asm volatile("barrier.cluster.wait;" ::: "memory");
 }
