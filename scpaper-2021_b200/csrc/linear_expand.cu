@@ -690,9 +690,9 @@ struct ExpandPlan {
 };
 
 // 4 bits: cycles of a K block for mb token blocks, fitted to B200 runs: 8192 -> 8192 at 64 features took 466 and 677
-// for one and two, at 128 features 690 (of expanding: 250 + 3.45 a feature), 916 and, for four, 1490: the thread that
-// issues products and commits bounds a block as long as there are several, the expansion where there is one.  (By the
-// products' 256 cycles alone, as the other formats are planned, 2000 tokens 8192 -> 8192 took 356 us for 225, 8192
+// for one and two, at 128 features 690 (of expanding: 250 + 3.45 a feature), 916 and, for four, 1490.  That is shared
+// memory's traffic, 107 to 146 bytes a cycle: a product reads 16 KB of activations and all the weights, copies and
+// expansion write both.  (By the products' 256 cycles alone, as the other formats are planned, 2000 tokens 8192 -> 8192 took 356 us for 225, 8192
 // tokens 4096 -> 4096 271 for 239.)
 long quant_cycles(int bn, int mb) {
     const long products = bn == 128 ? 342 + 287 * mb : 255 + 211 * mb, expand = 250 + bn * 7 / 2;
