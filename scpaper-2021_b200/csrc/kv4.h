@@ -64,7 +64,7 @@ inline int kv4_check_attention(const Kv4View& v, int batch, int seq, int nhead, 
     if (batch <= 0 || seq <= 0 || nhead <= 0 || max_len <= 0) return ET_ERR_INVALID_ARG;
     if (nhead % v.nkv || batch > 65535) return ET_ERR_SHAPE;
     const int64_t rows = static_cast<int64_t>(seq) * (nhead / v.nkv);
-    if (static_cast<int64_t>(batch) * seq > INT32_MAX || rows > INT32_MAX / 2 || (rows + 7) / 8 * v.nkv > 65535 ||
+    if (static_cast<int64_t>(batch) * seq > INT32_MAX || rows > INT32_MAX / 2 || (rows > 8 ? (rows + 15) / 16 : 1) * v.nkv > 65535 ||
         max_len > INT32_MAX - (1 << 20) || static_cast<int64_t>(batch) * seq * nhead > INT32_MAX)
         return ET_ERR_SHAPE;
     return ET_OK;

@@ -380,7 +380,8 @@ def test_attention_hidden_giants_cost_nothing(et, cuda, dh, mask_kind):
 
 @pytest.mark.parametrize("case", [(1, 40, 64, 1, 64, 64, 1024, [500]), (3, 1, 96, 3, 32, 128, 2048, [2049, 1, 4096]),
                                   (1, 200, 2, 2, 128, 128, 16, [201]), (2, 2, 4, 4, 16, 16, 16, [513, 1024]),
-                                  (200, 1, 2, 1, 64, 64, 16, list(range(1, 201)))], ids=str)
+                                  (200, 1, 2, 1, 64, 64, 16, list(range(1, 201))),
+                                  (1, 100000, 8, 8, 16, 16, 16, [40])], ids=lambda c: str(c)[:40])
 def test_attention_many_rows_large_pages_large_batches(et, cuda, case):
     _check_attention(et, cuda, *case, seed=17)
 

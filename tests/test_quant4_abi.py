@@ -98,6 +98,7 @@ def test_attention_refuses(et):
                     (dict(scale=inf), -1), (dict(scale=1e-30), -1), (dict(scale=1e30), -1),
                     (dict(scale=-1.0), -1), (dict(Q=0x5004), -2), (dict(Z=0x6008), -2),
                     (dict(batch=65536), -3), (dict(seq=1 << 22, batch=1), -3),
+                    (dict(seq=100000, batch=1, kind=7), -1),  # (the length is taken)
                     (dict(table_ld=4096, max_len=65536, ws=None), -6),
                     (dict(table_ld=4096, max_len=65536, bytes=64), -6),
                     (dict(table_ld=4096, max_len=65536, ws=0x10004), -2)):
