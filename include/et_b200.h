@@ -234,7 +234,9 @@ int et_1x16_densify(const int32_t* tile_idx, const int32_t* row_idx, const et_ha
  *   et_w4_densify dense[out, in] = fp16(c s + m), limited to +-65504, for et_linear_dense_fwd;
  *   et_linear_w4_fwd  the forward pass.  Few tokens: codes and fp16 activations are multiplied as they are,
  *     scales applied to fp32 sums (one pass over the 4-bit weights, no rounding of a weight); many tokens:
- *     the weights are expanded to fp16 operand tiles in shared memory in front of the tcgen05 product.
+ *     the weights are expanded to fp16 operand tiles in shared memory in front of the tcgen05 product, each
+ *     rounded to fp16 once and limited as et_w4_densify's (2^-11 of a weight at most; random signs leave
+ *     2.8e-4 of the result's norm where the result's own rounding is 2.1e-4).
  *     An activation that is not finite leaves no sum of its token finite (RELU then makes NaN 0).
  * codes, params, X, Y 16-byte aligned (bias: 2); in and out multiples of 16.  Like every weight, codes and
  * params must be complete (stream synchronised) before the first Linear call that uses them.  Stands beside

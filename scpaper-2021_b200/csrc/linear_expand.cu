@@ -181,8 +181,10 @@ struct PackedExpander {
 };
 
 // The same for 4-bit codes, a whole block of 16 rows x 128 features (two K blocks) at a time: every element is
-// written.  A code becomes fp16 exactly (1024 + c, less 1024), and c s + m is rounded to fp16 once: the tensor
-// core cannot scale its sums per group, so the operand has to carry the scale.  Lane 4 i + j expands the four
+// written.  A code becomes fp16 exactly (1024 + c, less 1024), and c s + m is rounded to fp16 once and limited to
+// 65504 (s is rounded, so 15 s + m may pass it, and an infinite weight would make NaN of a zero activation; only blocks
+// whose (s, m) can reach it pay for the limit: everywhere it cost 1 to 5 %): the tensor core cannot scale its sums per
+// group, so the operand has to carry the scale.  Lane 4 i + j expands the four
 // words of rows i and i + 8.  Blocks are copied asynchronously QUANT_AHEAD ahead into a ring of the warp's own (64 tokens
 // x 8192 -> 8192: 32 us; loads into registers, which are waited for together with younger ones, 33).  What
 // bounds it: quant_cycles below.
@@ -237,9 +239,12 @@ struct QuantExpander {
 #pragma unroll
             for (int n = 0; n < 4; ++n) sm[h][n] = p[(n << gb_log) >> 2];
         }
+        // (s, m) of the block's rows, once round: may a value pass the type's end?
+        const uint32_t* all = reinterpret_cast<const uint32_t*>(at + 1024);
+        const uint32_t last = (16u << gb_log) - 1;
+        const uint32_t big = q4::may_pass_end(all[lane & last]) | q4::may_pass_end(all[(lane + 32) & last]);
         __syncwarp();
         fetch(slot);
-        const __half2 base = __floats2half2_rn(1024.f, 1024.f);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int row = 8 * h + (lane >> 2), j = lane & 3;
@@ -251,13 +256,19 @@ struct QuantExpander {
                 const __half2 s = __low2half2(pair), m = __high2half2(pair);
                 uint32_t o[4];
 #pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    const uint32_t c = q4::and_or(words[n] >> (4 * p), q4::NIBBLES, 0x64006400u);
-                    const __half2 y = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), base), s, m);
-                    o[p] = *reinterpret_cast<const uint32_t*>(&y);
-                }
+                for (int p = 0; p < 4; ++p) o[p] = q4::unlimited2(words[n] >> (4 * p), s, m);
                 *reinterpret_cast<uint4*>(line + (n >> 1) * next_kb + ((((n & 1) * 4 + j) ^ (row & 7)) * 16)) =
                     make_uint4(o[0], o[1], o[2], o[3]);
+            }
+        }
+        if (__any_sync(0xffffffffu, big != 0)) {  // every lane limits what it wrote
+#pragma unroll 1
+            for (int k = 0; k < 8; ++k) {
+                const int row = 8 * (k >> 2) + (lane >> 2), n = k & 3, j = lane & 3;
+                uint4* to = reinterpret_cast<uint4*>(tile + row * 128 + (n >> 1) * next_kb +
+                                                     ((((n & 1) * 4 + j) ^ (row & 7)) * 16));
+                const uint4 w = *to;
+                *to = make_uint4(q4::limited2(w.x), q4::limited2(w.y), q4::limited2(w.z), q4::limited2(w.w));
             }
         }
     }

@@ -134,12 +134,28 @@ __device__ __forceinline__ uint32_t codes8(const uint4& v, uint32_t sm, float in
     return s > 0.f ? out : 0u;  // a constant group, or one that is not finite: 0
 }
 
-// fp16(c s + m), rounded once and limited to 65504 (s is rounded, so 15 s + m may pass it); NaN stays.
-__device__ __forceinline__ uint32_t value2(uint32_t code_pair, __half2 s, __half2 m) {
+// Nonzero where c s + m may pass the type's end for some code: |s| 2^11 or more, or |m| 2^15 or more (and for what is
+// not finite); below, |15 s + m| < 30720 + 32768.
+__device__ __forceinline__ uint32_t may_pass_end(uint32_t sm) {
+    return ((sm & 0x7fff7fffu) + 0x08001800u) & 0x80008000u;  // (the exponents carry)
+}
+
+// fp16(c s + m), rounded once.
+__device__ __forceinline__ uint32_t unlimited2(uint32_t code_pair, __half2 s, __half2 m) {
     const uint32_t c = and_or(code_pair, NIBBLES, 0x64006400u);
-    const __half2 base = __floats2half2_rn(1024.f, 1024.f), most = __floats2half2_rn(65504.f, 65504.f);
-    const __half2 v = __hmin2_nan(__hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), base), s, m), most);
+    const __half2 base = __floats2half2_rn(1024.f, 1024.f);
+    const __half2 v = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), base), s, m);
     return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Two values limited to 65504; NaN stays.
+__device__ __forceinline__ uint32_t limited2(uint32_t v) {
+    const __half2 most = __floats2half2_rn(65504.f, 65504.f);
+    const __half2 y = __hmin2_nan(*reinterpret_cast<const __half2*>(&v), most);
+    return *reinterpret_cast<const uint32_t*>(&y);
+}
+// fp16(c s + m), rounded once and limited (s is rounded, so 15 s + m may pass the type's end).
+__device__ __forceinline__ uint32_t value2(uint32_t code_pair, __half2 s, __half2 m) {
+    return limited2(unlimited2(code_pair, s, m));
 }
 
 // Eight values of a word whose value k is in nibble k, or (PAIRS) in (k >> 1) + 4 (k & 1).
