@@ -182,7 +182,7 @@ struct PackedExpander {
 
 // The same for 4-bit codes, a whole block of 16 rows x 128 features (two K blocks) at a time: every element is
 // written.  A code becomes fp16 exactly (1024 + c, less 1024), and c s + m is rounded to fp16 once and limited to
-// 65504 (s is rounded, so 15 s + m may pass it, and an infinite weight would make NaN of a zero activation; only blocks
+// +-65504 (s is rounded, so 15 s + m may pass it, and an infinite weight would make NaN of a zero activation; only blocks
 // whose (s, m) can reach it pay for the limit: everywhere it cost 1 to 5 %): the tensor core cannot scale its sums per
 // group, so the operand has to carry the scale.  Lane 4 i + j expands the four
 // words of rows i and i + 8.  Blocks are copied asynchronously QUANT_AHEAD ahead into a ring of the warp's own (64 tokens

@@ -147,10 +147,11 @@ __device__ __forceinline__ uint32_t unlimited2(uint32_t code_pair, __half2 s, __
     const __half2 v = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), base), s, m);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
-// Two values limited to 65504; NaN stays.
+// Two values limited to +-65504; NaN stays.  (s below 0 is nothing that the quantisers write, but arrays may come
+// from elsewhere.)
 __device__ __forceinline__ uint32_t limited2(uint32_t v) {
-    const __half2 most = __floats2half2_rn(65504.f, 65504.f);
-    const __half2 y = __hmin2_nan(*reinterpret_cast<const __half2*>(&v), most);
+    const __half2 most = __floats2half2_rn(65504.f, 65504.f), least = __floats2half2_rn(-65504.f, -65504.f);
+    const __half2 y = __hmax2_nan(__hmin2_nan(*reinterpret_cast<const __half2*>(&v), most), least);
     return *reinterpret_cast<const uint32_t*>(&y);
 }
 // fp16(c s + m), rounded once and limited (s is rounded, so 15 s + m may pass the type's end).

@@ -65,3 +65,34 @@ def test_linear_w4_weights_at_the_types_end(et, cuda, few, T, inn, out, group):
     tol = HALF * np.abs(want) + 2.0 ** -25 + err
     bad = ~(np.abs(y - want) <= tol)
     assert not bad.any(), (np.argwhere(bad)[:4], y[bad][:4], want[bad][:4])
+
+
+def test_values_are_limited_at_both_ends(et, cuda):
+    """Arrays that a caller fills may hold any finite (s, m): read back and made dense, values stay within +-65504."""
+    rng = _rng(2)
+    pairs = np.array([[4400, 0], [-4400, 0], [60000, -65504], [-60000, 65504], [-1, -65504], [1, 65504], [-65504, -65504],
+                      [65504, 65504]], np.float16)
+    c = rng.integers(0, 16, (16, 128)).astype(np.uint8)
+    c[:, ::9] = 15
+    sm = pairs[rng.integers(0, len(pairs), (16, 4))]
+    s, m = sm[..., 0], sm[..., 1]
+    want = ref.values(c, s, m).clip(-65504, 65504).astype(np.float16)
+    codes, params = ref.w4_arrays(c, s, m, 32)
+    q = et.W4Weight.from_arrays(_dev(codes, cuda), _dev(params, cuda), 128, 16, 32)
+    assert np.array_equal(q.densify().cpu().numpy(), want)
+    cache = et.KV4Cache(1, 16, 1, 128, 128, device=cuda)
+    for codes_, params_, rows in ((cache.k_codes, cache.k_params, ref.k_rows), (cache.v_codes, cache.v_params, ref.v_rows)):
+        codes_.copy_(_dev(rows(c)[None, None], cuda))
+        params_.copy_(_dev(sm[None, None], cuda))
+    k, v = et.kv4_read(cache, _dev(np.zeros((1, 1), np.int32), cuda), 1, 16)
+    assert np.array_equal(k.cpu().numpy(), want) and np.array_equal(v.cpu().numpy(), want)
+    # and the product over expanded weights sees no infinity
+    x = np.zeros((9, 128), np.float16)
+    x[np.arange(9), np.arange(9) * 14] = 2.0 ** -12
+    et.lib().et_debug_set_w4_few(0)
+    try:
+        y = et.linear_w4(_dev(x, cuda), q).cpu().numpy()
+    finally:
+        et.lib().et_debug_set_w4_few(-1)
+    assert np.array_equal(y, (want[:, np.arange(9) * 14].astype(np.float64).T * 2.0 ** -12).astype(np.float16))
+    assert et.device_error() == 0
