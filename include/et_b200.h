@@ -455,7 +455,7 @@ int et_kv4_read_fwd(const et_kv4_t* cache, et_half* K, et_half* V, int ldk, int 
  *   ET_MASK_CAUSAL    query i sees t <= kv_len[b] - q_len[b] + i: the queries are the newest tokens;
  *   ET_MASK_ADDITIVE  fp16 mask[seq, ldm] added to the scaled scores, ldm >= max_len.
  * A query that sees nothing (kv_len 0, or every score -inf) yields zeros.  What stands in a masked
- * place, NaN included, does not reach the output.
+ * place, NaN included, does not reach the output; a NaN that a query sees does, however small its weight.
  * max_len: the largest kv_len (at most table_ld * page); longer sequences are cut there and
  * reported (601).  scale: 2^-64 .. 2^64.  Q.K is exact up to fp32 sums (codes and fp16 queries are
  * multiplied as they are); a probability times its group's scale enters the second product with 22

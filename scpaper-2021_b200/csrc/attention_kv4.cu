@@ -457,6 +457,15 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
                 }
         }
 
+        uint32_t seen = 0;  // which of the scores are no -inf (an exponential of 0 may be a seen token's)
+        if (odd) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int k = 0; k < 4 * HALVES; ++k)
+                    if (x[k >> 2][t][(k >> 1) & 1][k & 1] != -INFINITY) seen |= 1u << (t * 4 * HALVES + k);
+        }
+
         // ---- online softmax.  The reference moves only when a score plus e passes it by 6: the lanes then need not agree
         // on the tile's maximum, and p s < 2^6 is as good to fp16.
         float mx[NT][2];
@@ -512,7 +521,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
 #pragma unroll
             for (int k = 0; k < 2 * HALVES; ++k)
                 px[k >> 1][t][k & 1] = pack_f32x2(x[k >> 1][t][k & 1][0], x[k >> 1][t][k & 1][1]);
-        if (odd) {  // a group of V that is not finite: NaN for the rows that see it, and for no other
+        if (odd) {  // a group of V that is not finite: NaN for the rows that see it, however little, and for no other
             const uint32_t* raw = reinterpret_cast<const uint32_t*>(st + 2 * S::CODES + S::PARAMS);
 #pragma unroll
             for (int k = 0; k < 2 * HALVES; ++k) {
@@ -526,8 +535,8 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
                     for (int t = 0; t < NT; ++t) {
                         float p0, p1;
                         unpack_f32x2(pm[g][t], p0, p1);
-                        if (x[k >> 1][t][k & 1][0] != 0.f) p0 = NAN;
-                        if (x[k >> 1][t][k & 1][1] != 0.f) p1 = NAN;
+                        if (seen >> (t * 4 * HALVES + 2 * k) & 1) p0 = NAN;
+                        if (seen >> (t * 4 * HALVES + 2 * k + 1) & 1) p1 = NAN;
                         pm[g][t] = pack_f32x2(p0, p1);
                     }
                 }
@@ -716,7 +725,7 @@ __global__ void __launch_bounds__(64) attention_kv4_join_kernel(const AttArgs a)
         for (int k = 0; k < JOIN_AHEAD; ++k) {
             const int s = s0 + k;
             const float f = __shfl_sync(0xffffffffu, s < 32 ? f0 : f1, s & 31);
-            if (f != 0.f && s < a.splits) {  // (0 also where the split saw nothing; NaN passes)
+            if (s < a.splits) {  // (a split that saw nothing has sums of 0; one far below the others may hold a NaN)
                 o.x = fmaf(v[k].x, f, o.x);
                 o.y = fmaf(v[k].y, f, o.y);
                 o.z = fmaf(v[k].z, f, o.z);

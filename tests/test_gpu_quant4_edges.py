@@ -96,3 +96,64 @@ def test_values_are_limited_at_both_ends(et, cuda):
         et.lib().et_debug_set_w4_few(-1)
     assert np.array_equal(y, (want[:, np.arange(9) * 14].astype(np.float64).T * 2.0 ** -12).astype(np.float16))
     assert et.device_error() == 0
+
+
+@pytest.mark.parametrize("where", ["first", "middle", "last"])
+@pytest.mark.parametrize("pattern", ["alone", "most"])
+@pytest.mark.parametrize("length,parts", [(100, 1), (900, 4), (9000, 36)])
+def test_attention_seen_nan_of_no_weight(et, cuda, length, parts, pattern, where):
+    """A NaN in V reaches the rows that see it whatever its weight, in one block, a cluster or two kernels: its score
+    lies 128 below the others' (e^-128 is no number of the exponential's), alone or with all tokens but the last 32."""
+    rng = _rng(length)
+    heads, dh, seq = 2, 64, 3
+    pages = (length + 15) // 16
+    cache = et.KV4Cache(pages, 16, heads, dh, dh, device=cuda)
+    need = cache.workspace_bytes(1, seq, heads, length)
+    assert (need > 0) == (parts > 4)
+    table = _dev(np.arange(pages, dtype=np.int32)[None], cuda)
+    k = rng.normal(0, 1, (length, heads * dh)).astype(np.float16)
+    v = rng.normal(0, 1, (length, heads * dh)).astype(np.float16)
+    at = {"first": 3, "middle": length // 2, "last": length - 2}[where]  # the last: hidden from query 0
+    low = np.zeros(length, bool)
+    low[at] = True
+    if pattern == "most":
+        low[: length - 32] = True
+    k[low] = -16.0
+    q = np.ones((seq, heads * dh), np.float16)
+    bad = v.copy()
+    bad[at, 70] = np.nan  # head 1, group 0
+    et.kv4_write(cache, _dev(k, cuda), _dev(bad, cuda), table, None, 1, length)
+    z = et.attention_kv4(cache, _dev(q, cuda), table, _dev(np.array([length], np.int32), cuda), 1, seq, heads, max_len=length)
+    assert et.device_error() == 0
+    z = z.cpu().numpy().astype(np.float64)
+    seen = np.zeros(z.shape, bool)
+    seen[[r for r in range(seq) if at <= length - seq + r], dh: dh + 32] = True
+    assert np.array_equal(np.isnan(z), seen), np.argwhere(np.isnan(z) != seen)[:4]
+    plain = [ref.values(*ref.quantise(x.reshape(length, heads, dh), 32)) for x in (k, v)]
+    for h in range(heads):
+        cols = slice(h * dh, (h + 1) * dh)
+        want = ref.attention(q[:, cols].astype(np.float64), plain[0][:, h], plain[1][:, h], length - seq + 1 + np.arange(seq),
+                             dh ** -0.5)
+        # scores: fp32 sums of dh products, twice (c s and m apart), of at most |k| <= 16 and |q| = 1
+        err = dh ** -0.5 * (dh + 8) * U32 * 2 * 16 * dh
+        tol = HALF * np.abs(want) + 2.0 ** -25 + 8.0 * (2 * err + 64 * U32 + length ** 0.5 * 8 * U32)
+        assert not (np.abs(z[:, cols] - want) > tol).any()
+
+
+def test_attention_masked_nan_is_hidden_whatever_its_score(et, cuda):
+    """-inf in an additive mask hides a NaN of V, the type's lowest value does not."""
+    rng = _rng(31)
+    length = 9000
+    cache = et.KV4Cache(563, 16, 1, 64, 64, device=cuda)
+    table = _dev(np.arange(563, dtype=np.int32)[None], cuda)
+    x = rng.normal(0, 1, (length, 64)).astype(np.float16)
+    x[5000, 40] = np.nan
+    et.kv4_write(cache, _dev(np.nan_to_num(x), cuda), _dev(x, cuda), table, None, 1, length)
+    q = _dev(rng.normal(0, 1, (2, 64)).astype(np.float16), cuda)
+    mask = np.zeros((2, length), np.float16)
+    mask[0, 5000], mask[1, 5000] = -np.inf, -65504.0
+    z = et.attention_kv4(cache, q, table, _dev(np.array([length], np.int32), cuda), 1, 2, 1, max_len=length,
+                         mask_kind=et.MASK_ADDITIVE, mask=_dev(mask, cuda)).cpu().numpy()
+    want = np.zeros((2, 64), bool)
+    want[1, 32:] = True
+    assert et.device_error() == 0 and np.array_equal(np.isnan(z), want)
