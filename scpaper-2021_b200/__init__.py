@@ -706,6 +706,8 @@ def attention_kv4(cache: "KV4Cache", q, table, kv_len, batch: int, seq: int, nhe
         z = empty_like(q) if whole and q_width == z_width else q.new_empty((rows, z_width))
     ldm = 0
     if mask is not None:
+        if mask_kind != MASK_ADDITIVE:
+            raise EtError("attention_kv4: a mask is read with MASK_ADDITIVE only")
         if mask.dim() != 2 or mask.shape[0] < seq or mask.shape[1] < max_len:
             raise EtError(f"attention_kv4: a mask [{seq}, {max_len}] is wanted")
         ldm = _row_stride(mask, mask.shape[1])

@@ -157,3 +157,18 @@ def test_attention_masked_nan_is_hidden_whatever_its_score(et, cuda):
     want = np.zeros((2, 64), bool)
     want[1, 32:] = True
     assert et.device_error() == 0 and np.array_equal(np.isnan(z), want)
+
+
+def test_mask_of_another_kind_is_refused(et, cuda):
+    """A mask that would not be read is refused, not dropped."""
+    import torch
+    cache = et.KV4Cache(4, 16, 2, 64, 64, device=cuda)
+    t = torch.zeros((1, 2), dtype=torch.int32, device=cuda)
+    n = torch.ones(1, dtype=torch.int32, device=cuda)
+    q = torch.zeros((1, 128), dtype=torch.float16, device=cuda)
+    mask = torch.zeros((1, 32), dtype=torch.float16, device=cuda)
+    for kw in ({}, {"mask_kind": et.MASK_CAUSAL}, {"mask_kind": et.MASK_NONE}):
+        with pytest.raises(et.EtError):
+            et.attention_kv4(cache, q, t, n, 1, 1, 2, mask=mask, **kw)
+    et.attention_kv4(cache, q, t, n, 1, 1, 2, mask=mask, mask_kind=et.MASK_ADDITIVE)
+    assert et.device_error() == 0
