@@ -1337,7 +1337,7 @@ class CachedStack:
             raise EtError(f"CachedStack: {longest} of {seq} new tokens")
         if self.used + longest > self.max_len:
             raise EtError(f"CachedStack: {self.used} + {longest} tokens do not fit into {self.max_len}")
-        # (all of it before the lengths move)
+        # (before the lengths move)
         _require("CachedStack", _types()[0], x)
         _check_rows("CachedStack", "x", x, self.batch * seq, self.layers[0].hidden)
         _check_pages("CachedStack", self.caches[0], self.batch, self.table, new_len)
@@ -1347,9 +1347,13 @@ class CachedStack:
         self.start.copy_(self.kv_len)
         self.kv_len.add_(seq if new_len is None else new_len.reshape(-1).clamp(0, seq))
         cur = x
-        for i, (layer, cache) in enumerate(zip(self.layers, self.caches)):
-            cur = layer.forward_cached(cur, buf[i & 1], cache, self.table, self.start, self.kv_len, self.batch, seq,
-                                       self.max_len, ws, new_len)
+        try:
+            for i, (layer, cache) in enumerate(zip(self.layers, self.caches)):
+                cur = layer.forward_cached(cur, buf[i & 1], cache, self.table, self.start, self.kv_len, self.batch, seq,
+                                           self.max_len, ws, new_len)
+        except EtError:  # what the library refuses (an x off a 16-byte boundary, a layer's description)
+            self.kv_len.copy_(self.start)
+            raise
         self.used += longest
         return cur
 

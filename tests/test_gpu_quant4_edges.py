@@ -172,3 +172,42 @@ def test_mask_of_another_kind_is_refused(et, cuda):
             et.attention_kv4(cache, q, t, n, 1, 1, 2, mask=mask, **kw)
     et.attention_kv4(cache, q, t, n, 1, 1, 2, mask=mask, mask_kind=et.MASK_ADDITIVE)
     assert et.device_error() == 0
+
+
+def _weights(et, seed, hidden, ff, qk=None):
+    qk = hidden if qk is None else qk
+    r = lambda n, shape, std: et.synth.normal(seed, n, shape, std)
+    w = {"wqkv": r(1, (2 * qk + hidden, hidden), 0.04), "bqkv": r(2, (2 * qk + hidden,), 0.1),
+         "wo": r(3, (hidden, hidden), 0.04), "bo": r(4, (hidden,), 0.1), "w1": r(5, (ff, hidden), 0.04),
+         "b1": r(6, (ff,), 0.1), "w2": r(7, (hidden, ff), 0.04), "b2": r(8, (hidden,), 0.1),
+         "ln1_g": 1 + r(9, (hidden,), 0.1), "ln1_b": r(10, (hidden,), 0.1), "ln2_g": 1 + r(11, (hidden,), 0.1),
+         "ln2_b": r(12, (hidden,), 0.1)}
+    return {k: np.asarray(v, np.float16) for k, v in w.items()}
+
+
+def test_cached_stack_keeps_its_lengths_when_a_layer_refuses(et, cuda):
+    """What only the library's own checks find - an x off a 16-byte boundary, a layer's weights - leaves the lengths
+    as they were, and the same tokens can be passed again."""
+    import torch
+    hidden, batch, seq = 128, 2, 6
+    layers = [et.EncoderLayer(_weights(et, 51 + i, hidden, 256), 2, et.ACT_GELU) for i in range(2)]
+    stack = et.CachedStack(layers, batch, 33, page=16, device=cuda)
+    x = _dev(_rng(19).normal(0, 1, (batch * seq, hidden)).astype(np.float16), cuda)
+    first = stack.forward(x, seq).clone()
+    want = stack.forward(x, seq).clone()
+    stack.reset()
+    assert torch.equal(stack.forward(x, seq), first)
+    wide = torch.zeros(batch * seq * hidden + 8, dtype=torch.float16, device=cuda)
+    off = wide[1: 1 + batch * seq * hidden].view(batch * seq, hidden)
+    off.copy_(x)
+    assert off.is_contiguous() and off.data_ptr() % 16
+    with pytest.raises(et.EtError):
+        stack.forward(off, seq)
+    assert stack.kv_len.tolist() == [seq, seq] and stack.used == seq
+    kept = layers[1].desc.ln1_gamma
+    layers[1].desc.ln1_gamma = None  # the second layer refuses, after the first has run
+    with pytest.raises(et.EtError):
+        stack.forward(x, seq)
+    layers[1].desc.ln1_gamma = kept
+    assert stack.kv_len.tolist() == [seq, seq] and stack.used == seq
+    assert torch.equal(stack.forward(x, seq), want) and et.device_error() == 0
