@@ -356,6 +356,82 @@ int after_attention(const et_encoder_layer_t* layer, const LayerBuffers& b, cons
     return ffn_block(layer, b, T, out, s);
 }
 
+// What run_linear answers for these weights over T rows of this file's (aligned) buffers, without launching.
+int check_linear(const et_linear_t& lin, int T) {
+    const int n = lin.nnz_tiles;
+    const bool bias_ok = aligned16(lin.bias), weight_ok = aligned16(lin.weight);  // (null is aligned)
+    if (lin.format == ET_FMT_DENSE) {
+        if (!lin.weight) return ET_ERR_INVALID_ARG;
+        if (!weight_ok || !bias_ok) return ET_ERR_ALIGNMENT;
+        return lin.in % 8 || lin.out % 8 ? ET_ERR_SHAPE : ET_OK;
+    }
+    if (n < 0) return ET_ERR_INVALID_ARG;
+    const bool stored = n > 0, indexed = lin.row_off && lin.weight;
+    switch (lin.format) {
+        case ET_FMT_W4:  // (sizes and null pointers: check_layer)
+            if (T > 65535 * 128) return ET_ERR_SHAPE;
+            return weight_ok && aligned16(lin.row_ptr) ? ET_OK : ET_ERR_ALIGNMENT;
+        case ET_FMT_1X16:
+            if (!lin.row_ptr || (stored && !indexed)) return ET_ERR_INVALID_ARG;
+            if (lin.in % 16 || lin.out % 16 || T > 65535 * 128) return ET_ERR_SHAPE;
+            return weight_ok ? ET_OK : ET_ERR_ALIGNMENT;
+        case ET_FMT_CSR:
+            if (!lin.row_ptr || (stored && !indexed)) return ET_ERR_INVALID_ARG;
+            return lin.in % 8 || lin.in > 8192 ? ET_ERR_SHAPE : ET_OK;
+        case ET_FMT_ROW:
+            if (stored && (!lin.row_ptr || !lin.weight)) return ET_ERR_INVALID_ARG;
+            if (lin.in % 16 || lin.out % 16) return ET_ERR_SHAPE;
+            return bias_ok && (!stored || weight_ok) ? ET_OK : ET_ERR_ALIGNMENT;
+        case ET_FMT_COL:
+            if (!lin.row_ptr || !lin.weight || !stored) return ET_ERR_INVALID_ARG;
+            if (lin.in % 16 || lin.out % 16 || n % 8) return ET_ERR_SHAPE;
+            return bias_ok && weight_ok ? ET_OK : ET_ERR_ALIGNMENT;
+        case ET_FMT_TILE:
+        case ET_FMT_TILE_PACKED:
+            if (!lin.row_ptr || (stored && !lin.weight)) return ET_ERR_INVALID_ARG;
+            if (stored && (lin.format == ET_FMT_TILE ? !lin.row_off : !lin.pk_mask || !lin.pk_off)) return ET_ERR_INVALID_ARG;
+            if (lin.in % 16 || lin.out % 16 || lin.in > 8192) return ET_ERR_SHAPE;
+            return bias_ok && weight_ok ? ET_OK : ET_ERR_ALIGNMENT;
+        default: return ET_ERR_INVALID_ARG;
+    }
+}
+
+// The same for the two Linears that a LayerNorm follows: where both run as one kernel it reads bias, gamma and beta
+// one element at a time.  `dense` with K: the product that the weights amount to (ffn_block).
+int check_linear_ln(const et_linear_t& lin, bool dense, int K, const et_half* gamma, const et_half* beta, int bit,
+                    int hidden, int T) {
+    if (dense) {
+        if (!lin.weight) return ET_ERR_INVALID_ARG;
+        if (!aligned16(lin.weight)) return ET_ERR_ALIGNMENT;
+        if (K % 8 || hidden % 8) return ET_ERR_SHAPE;
+        if (aligned16(lin.bias) && aligned16(gamma) && aligned16(beta)) return ET_OK;
+        return ln_fused(bit, T, hidden, K) && gemm_ln_applies(T, hidden, K) ? ET_OK : ET_ERR_ALIGNMENT;
+    }
+    const int st = check_linear(lin, T);
+    if (st != ET_OK) return st;
+    if (hidden % 8) return ET_ERR_SHAPE;
+    return aligned16(gamma) && aligned16(beta) ? ET_OK : ET_ERR_ALIGNMENT;
+}
+
+// The layer's weights, as far as the calls that use them would refuse them.
+int check_weights(const et_encoder_layer_t* L, int T) {
+    int st = check_linear(L->qkv, T);
+    if (st != ET_OK) return st;
+    if ((st = check_linear_ln(L->o, L->o.format == ET_FMT_DENSE, L->vdim, L->ln1_gamma, L->ln1_beta, 1, L->hidden, T)) !=
+        ET_OK)
+        return st;
+    const bool pair = ffn_is_compressed_pair(L);
+    if (pair) {  // (a dense product over the kept rows, whose bias is chosen by the same list)
+        if (!L->ffn1.weight) return ET_ERR_INVALID_ARG;
+        if (!aligned16(L->ffn1.weight) || !aligned16(L->ffn1.bias)) return ET_ERR_ALIGNMENT;
+        if (L->hidden % 8) return ET_ERR_SHAPE;
+    } else if ((st = check_linear(L->ffn1, T)) != ET_OK) {
+        return st;
+    }
+    return check_linear_ln(L->ffn2, pair || L->ffn2.format == ET_FMT_DENSE, pair ? L->ffn1.nnz_tiles : L->ff,
+                           L->ln2_gamma, L->ln2_beta, 2, L->hidden, T);
+}
+
 // Layer and cache describe the same heads.
 int check_cached(const et_encoder_layer_t* L, const et_kv4_t* c) {
     const int st = check_layer(L);
@@ -459,6 +535,7 @@ int et_encoder_layer_cached_fwd(const et_encoder_layer_t* layer, const et_kv4_t*
     if (!workspace) return ET_ERR_WORKSPACE;
     if (reinterpret_cast<uintptr_t>(workspace) & 255u) return ET_ERR_ALIGNMENT;
     if (!et::aligned16(x) || !et::aligned16(out)) return ET_ERR_ALIGNMENT;
+    if ((st = et::check_weights(layer, batch * seq)) != ET_OK) return st;
     const et::LayerBuffers b = et::carve(layer, batch, seq, workspace);
     const size_t att = et_attention_kv4_workspace_bytes(cache, batch, seq, layer->nhead, max_len);
     if (workspace_bytes < b.total + et::align256(att)) return ET_ERR_WORKSPACE;

@@ -211,3 +211,31 @@ def test_cached_stack_keeps_its_lengths_when_a_layer_refuses(et, cuda):
     layers[1].desc.ln1_gamma = kept
     assert stack.kv_len.tolist() == [seq, seq] and stack.used == seq
     assert torch.equal(stack.forward(x, seq), want) and et.device_error() == 0
+
+
+@pytest.mark.parametrize("batch", [2, 130])
+def test_cached_layer_takes_vectors_off_a_boundary(et, cuda, batch):
+    """Where a Linear and its LayerNorm run as one kernel, bias, gamma and beta may lie anywhere: such layers are taken."""
+    import torch
+    from conftest import assert_close
+    hidden, ff, nhead = 256, 512, 4
+    w = _weights(et, 81, hidden, ff)
+    layers = [et.EncoderLayer(w, nhead, et.ACT_GELU) for _ in range(2)]
+    keep = []
+
+    def off(name, size):
+        t = torch.zeros(size + 8, dtype=torch.float16, device=cuda)
+        t[1: 1 + size] = _dev(w[name], cuda)
+        keep.append(t)
+        return t.data_ptr() + 2
+
+    d = layers[1].desc
+    d.ln1_gamma, d.ln1_beta, d.ln2_gamma, d.ln2_beta = (off(n, hidden) for n in ("ln1_g", "ln1_b", "ln2_g", "ln2_b"))
+    d.o.bias, d.ffn2.bias = off("bo", hidden), off("b2", hidden)
+    x = _dev(_rng(3).normal(0, 1, (batch, hidden)).astype(np.float16), cuda)
+    outs = []
+    for layer in layers:
+        stack = et.CachedStack([layer], batch, 16, page=16, device=cuda)
+        outs.append(stack.forward(x, 1).clone())
+    assert_close(outs[1].cpu().numpy(), outs[0].cpu().numpy(), "off a boundary")
+    assert et.device_error() == 0

@@ -205,3 +205,63 @@ def test_python_wrappers_refuse_host_tensors(et):
         pytest.skip("the CPU suite's case")
     with pytest.raises(Exception):
         et.W4Weight(torch.zeros((16, 128), dtype=torch.float16))
+
+
+def test_cached_layer_refuses_its_weights_before_the_cache_is_written(et):
+    """What a later product of the layer would refuse is found before the projection and the cache's write are
+    launched, for every weight format and with the status of the product's own call."""
+    lib = et.lib()
+    d = et.EncoderLayerDesc()
+    dims = (("qkv", 256, 768), ("o", 256, 256), ("ffn1", 256, 512), ("ffn2", 512, 256))
+    for n, (name, inn, out) in enumerate(dims):
+        lin = getattr(d, name)
+        lin.in_, lin.out, lin.weight, lin.bias = inn, out, 0x100000 * (n + 1), None
+    for n, name in enumerate(("ln1_gamma", "ln1_beta", "ln2_gamma", "ln2_beta")):
+        setattr(d, name, 0x10000 * (n + 1))
+    d.hidden, d.nhead, d.kdim, d.vdim, d.ff, d.act = 256, 4, 256, 256, 512, 2
+    c = _cache(et)
+    before = lib.et_launch_count()
+
+    def fwd():
+        return lib.et_encoder_layer_cached_fwd(P(ctypes.addressof(d)), ctypes.byref(c), P(0x2000000), P(0x3000000), 2, 1,
+                                               P(0x7000), 4, P(0x8000), P(0x9000), None, 64, P(0x40000000), Z(1 << 40), None)
+
+    arrays = dict(row_ptr=0x700000, row_off=0x710000, weight=0x720000, pk_mask=0x730000, pk_off=0x740000)
+    wrong = {et.FMT_DENSE: ((dict(weight=None), -1), (dict(weight=0x720008), -2)),
+             et.FMT_W4: ((dict(weight=0x720008), -2), (dict(row_ptr=0x700004), -2), (dict(row_ptr=None), -1)),
+             et.FMT_1X16: ((dict(row_ptr=None), -1), (dict(row_off=None), -1), (dict(weight=0x720002), -2)),
+             et.FMT_CSR: ((dict(row_ptr=None), -1), (dict(weight=None), -1), (dict(nnz_tiles=-1), -1)),
+             et.FMT_ROW: ((dict(row_ptr=None), -1), (dict(weight=0x720008), -2), (dict(bias=0x720002), -2)),
+             et.FMT_COL: ((dict(nnz_tiles=0), -1), (dict(nnz_tiles=60), -3), (dict(weight=0x720008), -2),
+                          (dict(bias=0x720002), -2)),
+             et.FMT_TILE: ((dict(row_off=None), -1), (dict(weight=0x720008), -2), (dict(bias=0x720002), -2)),
+             et.FMT_TILE_PACKED: ((dict(pk_mask=None), -1), (dict(pk_off=None), -1), (dict(weight=0x720008), -2)),
+             99: ((dict(), -1),)}
+    for name, inn, out in dims[1:]:  # (the projection is the first to run in any case)
+        lin = getattr(d, name)
+        for fmt, cases in wrong.items():
+            for bad, status in cases:
+                for k, v in {**arrays, "bias": None, "nnz_tiles": 64, **bad}.items():
+                    setattr(lin, k, v)
+                lin.format = fmt
+                assert fwd() == status, (name, fmt, bad)
+        lin.format, lin.weight, lin.bias = et.FMT_DENSE, 0x720000, None
+    for name in ("ln1_gamma", "ln1_beta", "ln2_gamma", "ln2_beta"):
+        kept = getattr(d, name)
+        for lin, fmt in ((d.o, et.FMT_1X16), (d.ffn2, et.FMT_1X16)):  # (no dense product: the LayerNorm runs by itself)
+            lin.format, lin.nnz_tiles, lin.row_ptr, lin.row_off = fmt, 64, 0x700000, 0x710000
+        setattr(d, name, kept + 2)
+        assert fwd() == -2, name
+        setattr(d, name, kept)
+    # pruned hidden units: the pair runs as two dense products
+    for lin, fmt in ((d.ffn1, et.FMT_ROW), (d.ffn2, et.FMT_COL)):
+        lin.format, lin.nnz_tiles, lin.row_ptr, lin.weight, lin.bias = fmt, 64, 0x700000, 0x720000, None
+    for lin, bad, status in ((d.ffn1, dict(weight=None), -1), (d.ffn1, dict(bias=0x720008), -2),
+                             (d.ffn2, dict(weight=0x720008), -2)):
+        kept = {k: getattr(lin, k) for k in bad}
+        for k, v in bad.items():
+            setattr(lin, k, v)
+        assert fwd() == status, bad
+        for k, v in kept.items():
+            setattr(lin, k, v)
+    assert lib.et_launch_count() == before
