@@ -239,3 +239,146 @@ def test_cached_layer_takes_vectors_off_a_boundary(et, cuda, batch):
         outs.append(stack.forward(x, 1).clone())
     assert_close(outs[1].cpu().numpy(), outs[0].cpu().numpy(), "off a boundary")
     assert et.device_error() == 0
+
+
+FORMATS = ["dense", "tile", "tile_packed", "1x16", "csr", "row", "col", "w4", "pair"]
+
+
+def _in_format(et, cuda, w, fmt):
+    """The weights pruned for a format, the layer in it, and the projection as an operator of its own."""
+    import torch
+    synth = et.synth
+    w = dict(w)
+    names = ("wqkv", "wo", "w1", "w2")
+    out, ff = w["wqkv"].shape[0], w["w1"].shape[0]
+    bias = _dev(w["bqkv"], cuda)
+    keep = {n: np.ascontiguousarray(synth.choose_ids(7, i, w[n].shape[0 if fmt == "row" else 1], 0.5)).astype(np.int32)
+            for i, n in enumerate(names)}
+    hidden_units = keep["w2"]
+    for i, n in enumerate(names):
+        m = np.zeros_like(w[n])
+        if fmt in ("tile", "tile_packed"):
+            w[n] = np.asarray(synth.prune_tiles(w[n], 3, i, 0.5), np.float16)
+        elif fmt in ("1x16", "csr"):
+            w[n] = np.asarray(synth.prune_1x16(w[n], 3, i, 0.5), np.float16)
+        elif fmt == "row":
+            m[keep[n]] = w[n][keep[n]]
+            w[n] = m
+        elif fmt == "col":
+            m[:, keep[n]] = w[n][:, keep[n]]
+            w[n] = m
+    if fmt == "pair":  # pruned hidden units of the feed-forward block
+        m = np.zeros_like(w["w2"])
+        m[:, hidden_units] = w["w2"][:, hidden_units]
+        w["w2"] = m
+    ids = lambda n: _dev(keep[n], cuda)
+    d = lambda a: _dev(np.asarray(a), cuda)
+    if fmt in ("tile", "tile_packed"):
+        layer = et.EncoderLayer(w, 4, et.ACT_GELU, tile_sparse="unpacked" if fmt == "tile" else "packed")
+        rp, ro, tiles = synth.dense_to_tile(w["wqkv"])
+        if fmt == "tile":
+            a = [d(rp), d(ro), d(tiles)]
+            project = lambda x: et.linear_tile(x, *a, out, bias)
+        else:
+            pk = et.PackedTiles(rp, ro, tiles, w["wqkv"].shape[1], out, cuda)
+            project = lambda x: et.linear_tile_packed(x, pk, bias)
+    elif fmt in ("1x16", "csr"):
+        layer = et.EncoderLayer(w, 4, et.ACT_GELU, formats={n: fmt for n in names})
+        a = [d(v) for v in (synth.dense_to_1x16 if fmt == "1x16" else synth.dense_to_csr)(w["wqkv"])]
+        op = et.linear_1x16 if fmt == "1x16" else et.linear_csr
+        project = lambda x: op(x, *a, out, bias)
+    elif fmt == "row":
+        layer = et.EncoderLayer(w, 4, et.ACT_GELU, formats={n: ("row", keep[n]) for n in names})
+        rows, of = d(w["wqkv"][keep["wqkv"]]), ids("wqkv")
+        project = lambda x: et.linear_row(x, of, rows, out, bias)
+    elif fmt == "col":
+        layer = et.EncoderLayer(w, 4, et.ACT_GELU, formats={n: ("col", keep[n]) for n in names})
+        cols, of = d(w["wqkv"][:, keep["wqkv"]]), ids("wqkv")
+        project = lambda x: et.linear_col(x, of, cols, bias)
+    elif fmt == "w4":
+        layer = et.EncoderLayer(w, 4, et.ACT_GELU, formats={n: "w4" for n in names})
+        q = {n: et.W4Weight(d(w[n]), 128) for n in names}
+        project = lambda x: et.linear_w4(x, q["wqkv"], bias)
+        for n in names:
+            w[n] = q[n].densify().cpu().numpy()
+    else:
+        formats = {"w1": ("row", hidden_units), "w2": ("col", hidden_units)} if fmt == "pair" else {}
+        layer = et.EncoderLayer(w, 4, et.ACT_GELU, formats=formats)
+        dense = d(w["wqkv"])
+        project = lambda x: et.linear_dense(x, dense, bias)
+    return w, layer, project
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_cached_layer_in_every_format(et, cuda, fmt):
+    """A prompt in two chunks of up to 50 tokens (the second on top of cached ones, across pages, one sequence a token
+    short), then two single tokens: the cache to the bit of the format's own projection, what follows to the path's
+    tolerance of the same layer in dense weights."""
+    import torch
+    from conftest import assert_close
+    hidden, ff, nhead, batch, page, per = 256, 512, 4, 2, 16, 7
+    most = page * per
+    w, layer, project = _in_format(et, cuda, _weights(et, 71, hidden, ff), fmt)
+    dev = {k: _dev(v, cuda) for k, v in w.items()}
+    caches = [et.KV4Cache(batch * per, page, nhead, 64, 64, device=cuda) for _ in range(2)]
+    table = _dev(_rng(1).permutation(batch * per).reshape(batch, per).astype(np.int32), cuda)
+    kv = torch.zeros(batch, dtype=torch.int32, device=cuda)
+    for step, (seq, new) in enumerate(((50, [50, 49]), (50, [49, 50]), (1, None), (1, None))):
+        n = None if new is None else _dev(np.array(new, np.int32), cuda)
+        x = _dev(_rng(step).normal(0, 1, (batch * seq, hidden)).astype(np.float16), cuda)
+        start = kv.clone()
+        kv += 1 if new is None else n
+        assert int(kv.max()) <= most
+        ws = torch.empty(layer.cached_workspace_bytes(caches[0], batch, seq, most), dtype=torch.uint8, device=cuda)
+        out = torch.empty_like(x)
+        layer.forward_cached(x, out, caches[0], table, start, kv, batch, seq, most, ws, n)
+        qkv = project(x)
+        et.kv4_write(caches[1], qkv[:, hidden: 2 * hidden], qkv[:, 2 * hidden:], table, start, batch, seq, new_len=n)
+        for a in ("k_codes", "k_params", "v_codes", "v_params"):
+            assert torch.equal(getattr(caches[0], a), getattr(caches[1], a)), (step, a)
+        z = et.attention_kv4(caches[1], qkv[:, :hidden], table, kv, batch, seq, nhead, max_len=most, q_len=n)
+        y = et.skip_layernorm(et.linear_dense(z, dev["wo"], dev["bo"]), x, dev["ln1_g"], dev["ln1_b"])
+        f = et.linear_dense(y, dev["w1"], dev["b1"], et.ACT_GELU)
+        want = et.skip_layernorm(et.linear_dense(f, dev["w2"], dev["b2"]), y, dev["ln2_g"], dev["ln2_b"])
+        assert et.device_error() == 0
+        live = np.concatenate([np.arange(seq) < (seq if new is None else new[b]) for b in range(batch)])
+        assert_close(out.cpu().numpy()[live], want.cpu().numpy()[live], f"{fmt} step {step}")
+
+
+@pytest.mark.parametrize("ratio", [2.0 ** -8, 2.0 ** -12])
+@pytest.mark.parametrize("seq", [1, 12])
+def test_attention_groups_of_unequal_size(et, cuda, seq, ratio):
+    """Groups of a head whose ranges differ: p s enters the second product as two fp16 numbers, so to 2^-22 of itself or
+    to 2^-24 of the row's largest over all groups, times a code's distance from 8; the sums' share as ever."""
+    rng = _rng(seq)
+    length, heads, dh = 300, 2, 128
+    cache = et.KV4Cache(19, 16, heads, dh, dh, device=cuda)
+    table = _dev(np.arange(19, dtype=np.int32)[None], cuda)
+    k = rng.normal(0, 1, (length, heads * dh)).astype(np.float16)
+    v = rng.normal(0, 1, (length, heads, 4, 32)) * ratio ** np.array([0, 1, 0.5, 1])[:, None]
+    v = v.reshape(length, heads * dh).astype(np.float16)
+    q = rng.normal(0, 1, (seq, heads * dh)).astype(np.float16)
+    et.kv4_write(cache, _dev(k, cuda), _dev(v, cuda), table, None, 1, length)
+    z = et.attention_kv4(cache, _dev(q, cuda), table, _dev(np.array([length], np.int32), cuda), 1, seq, heads,
+                         max_len=length, mask_kind=et.MASK_NONE).cpu().numpy().astype(np.float64)
+    assert et.device_error() == 0
+    (ck, sk, mk), (cv, sv, mv) = (ref.quantise(x.reshape(length, heads, dh), 32) for x in (k, v))
+    k64, v64 = ref.values(ck, sk, mk), ref.values(cv, sv, mv)
+    sv, mv = sv.astype(np.float64), mv.astype(np.float64)
+    for h in range(heads):
+        qq = q[:, h * dh: (h + 1) * dh].astype(np.float64)
+        score = qq @ k64[:, h].T * dh ** -0.5
+        p = np.exp(score - score.max(-1, keepdims=True))
+        p /= p.sum(-1, keepdims=True)
+        big_k = float((16 * sk[:, h] + np.abs(mk[:, h])).max())
+        err = dh ** -0.5 * (dh + 8) * U32 * big_k * np.abs(qq).sum(-1, keepdims=True)
+        for g in range(4):
+            cols = slice(32 * g, 32 * g + 32)
+            want = p @ v64[:, h, cols]
+            ps = p * sv[:, h, g]
+            largest = (p[..., None] * sv[:, h]).max((1, 2))[:, None]
+            halves = 8 * np.maximum(2.0 ** -22 * ps, 2.0 ** -24 * largest).sum(-1, keepdims=True)
+            size = (p * (8 * sv[:, h, g] + np.abs(mv[:, h, g] + 8 * sv[:, h, g]))).sum(-1, keepdims=True)
+            tol = HALF * np.abs(want) + 2.0 ** -25 + halves + size * (2 * err + (64 + length) * U32)
+            off = np.abs(z[:, h * dh + 32 * g: h * dh + 32 * g + 32] - want)
+            assert not (off > tol).any(), (h, g, off.max(), tol.min())
