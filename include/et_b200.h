@@ -457,10 +457,11 @@ int et_kv4_read_fwd(const et_kv4_t* cache, et_half* K, et_half* V, int ldk, int 
  * A query that sees nothing (kv_len 0, or every score -inf) yields zeros.  What stands in a masked
  * place, NaN included, does not reach the output; a NaN that a query sees does, however small its weight.
  * max_len: the largest kv_len (at most table_ld * page); longer sequences are cut there and
- * reported (601).  scale: 2^-64 .. 2^64.  Q.K is exact up to fp32 sums (codes and fp16 queries are
- * multiplied as they are); a probability times its group's scale enters the second product with 22
- * bits, or to 2^-25 of the row's largest such product (groups of a head whose ranges lie 2^10 and
- * more apart: the small ones are as precise as the large ones allow).
+ * reported (601).  scale: 2^-64 .. 2^64.  Codes and fp16 queries are multiplied as they are, with
+ * fp32 sums; only where a row's largest |q| is 2^11 or more, values below 2^-23 of it are rounded,
+ * by 2^-35 of it at most.  A probability times its group's scale enters the
+ * second product with 22 bits, or to 2^-24 of the row's largest such product (groups of a head
+ * whose ranges lie 2^10 and more apart: the small ones are as precise as the large ones allow).
  * The long axis is split over thread blocks when there are few rows; their fp32 partial results
  * go to the workspace (et_attention_kv4_workspace_bytes; 0: none needed), which calls that may
  * overlap on the GPU must not share.  Nothing of it has to be set or kept.  */

@@ -298,8 +298,10 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm(NG, NT)) attention_kv4_
 #pragma unroll
     for (int n = 0; n < STAGES - 1; ++n) issue(n);
 
-    // ---- the rows' queries, scaled by a power of two of their own to at most 2^11: lossless, and room for the
-    // factor 16 that makes up for the nibbles which K's codes are multiplied at (4 bits up, every second pair)
+    // ---- the rows' queries, scaled by a power of two of their own to at most 2^11: room for the factor 16 that makes
+    // up for the nibbles which K's codes are multiplied at (4 bits up, every second pair).  Lossless where the row's
+    // largest is below 2^11; above, the power is 2^-1 to 2^-5, and what falls below the type's normal numbers is rounded
+    // to its grid of 2^-24: by 2^-25, 2^-35 of the largest (a score's fp32 sums are off by 2^-23 of their own sizes)
     int limit[NT][2];     // tokens that rows 8 t + 2 j, 8 t + 2 j + 1 see
     uint64_t qs[NG][NT];  // rows 8 t + 2 j, + 1: sums over the group, in the units of the first product
     float unit[NT][2];    // those units times scale and log2(e)
