@@ -239,7 +239,8 @@ int et_1x16_densify(const int32_t* tile_idx, const int32_t* row_idx, const et_ha
  *     2.8e-4 of the result's norm where the result's own rounding is 2.1e-4).
  *     An activation that is not finite leaves no sum of its token finite (RELU then makes NaN 0).
  * codes, params, X, Y 16-byte aligned (bias: 2); in and out multiples of 16.  Like every weight, codes and
- * params must be complete (stream synchronised) before the first Linear call that uses them.  Stands beside
+ * params must be complete (stream synchronised) before the first Linear call that uses them; arrays from elsewhere
+ * keep c s + m inside +-65504, as et_w4_pack's do up to the rounding of s.  Stands beside
  * the weight formats of mat_type/; the reference has no quantised one. */
 int et_w4_sizes(int in, int out, int group, size_t* code_bytes, size_t* param_bytes);
 int et_w4_pack(const et_half* W, int in, int out, int group, uint8_t* codes, et_half* params, et_stream stream);

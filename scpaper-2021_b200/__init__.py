@@ -404,7 +404,9 @@ def _types():
 class W4Weight:
     """A Linear weight in 4 bits: codes and one fp16 (scale, minimum) pair per `group` input features of an output
     row (32, 64 or 128), quantised on the GPU from a dense W[out, in].  from_arrays() takes the two arrays in
-    the layout that et_b200.h states instead."""
+    the layout that et_b200.h states instead: complete, like every weight, before the first linear_w4 (kernels fetch
+    weights ahead of their predecessors on the stream), and with c s + m inside +-65504 (beyond, the expanded form of many
+    tokens is limited there and the form of few tokens is not)."""
 
     def __init__(self, w, group: int = 128):
         import torch

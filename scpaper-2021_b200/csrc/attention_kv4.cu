@@ -20,13 +20,16 @@
 // shared memory, or (more than 4) to blocks that leave them to a second kernel.
 //
 // Layout.  Both products have the cache as their 16-row operand and eight query rows as their 8-column one: a few
-// rows then waste little of the tensor core and of the registers (with the rows on the 16 side, half
-// empty, the accumulators took 64 registers a thread instead of 32 at 128 features, and spilled).  Lane 4 i + j holds
+// rows then waste less of the tensor core and of the registers (with the rows on the 16 side, half
+// empty, the accumulators took 64 registers a thread instead of 32 at 128 features; as it is, 96 and 128 features spill 12 to
+// 76 bytes of loads a thread, two row tiles of 128 features 276: at 4 x 32768 tokens, 128 features, 1.3 % of the instructions).  Lane 4 i + j holds
 // word j of every group of token tau(i) = (i >> 1) + 4 (i & 1) of K, and unit i of every group of tokens j, j + 4,
 // j + 8, j + 12 of V: the order in which the transposed probabilities (movmatrix) lie along the second product.
 //
-// What bounds it: instruction issue.  Unpacking alone takes 1.25 instructions per element and lane (a shift and
-// an AND for two codes, a subtraction for V's), scales and the softmax as much again.
+// What bounds it: instruction issue (four warps a scheduler issue in 50 % of the cycles at 16 x 2000 tokens of 64 features,
+// 57 % at 4 x 32768 of 128).  Unpacking alone takes 1.25 instructions per element and lane (a shift and
+// an AND for two codes, a subtraction for V's), scales and the softmax as much again; these run for eight rows
+// whether there are that many or not (one token of heads of their own: one of eight).
 #include "kernels.h"
 #include "kv4.h"
 #include "quant4.cuh"
