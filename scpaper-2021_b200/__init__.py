@@ -685,7 +685,7 @@ def kv4_read(cache: "KV4Cache", table, batch: int, seq: int, start=None, length=
 def attention_kv4(cache: "KV4Cache", q, table, kv_len, batch: int, seq: int, nhead: int, max_len=None,
                   mask_kind=MASK_CAUSAL, mask=None, q_len=None, scale=None, out=None, workspace=None):
     """softmax(q k^T * scale + mask) v of q [batch * seq, nhead * dh_qk] over the kv_len[b] cached tokens of every
-    sequence, the queries' own (its newest, written first) included.  max_len: the largest kv_len (the page
+    sequence, the queries' own (its newest, written first) included.  max_len: the largest kv_len, 1 or more (the page
     table's reach where None); a tight one lets the call split the sequence well.  q_len[b] < seq: padding rows,
     left as they were (zeros where `out` is None).  mask: fp16 [seq, >= max_len] for MASK_ADDITIVE.  workspace:
     optional scratch of cache.workspace_bytes(...) bytes, not shared with calls that may overlap."""
